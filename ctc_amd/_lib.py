@@ -17,6 +17,8 @@ SYMBOLS = (
     "ctc_tc_plan_shard", "ctc_tc_plan_gemm_plan", "ctc_tc_plan_prepare", "ctc_tc_execute", "ctc_tc_permute",
     "ctc_tc_ttgt_workspace_bytes", "ctc_tc_execute_ttgt", "ctc_tc_fill", "ctc_tc_time_execute", "ctc_tc_time_execute_each",
     "ctc_tc_grouped_contract", "ctc_tc_execute_noalloc", "ctc_tc_noalloc_scratch_bytes", "ctc_tc_set_option", "ctc_tc_get_option",
+    "ctc_tc_block_quantize", "ctc_tc_scaled_workspace_bytes", "ctc_tc_scaled_contract", "ctc_tc_scaled_grouped_contract",
+    "ctc_tc_expert_workspace_bytes", "ctc_tc_expert_layer",
 )
 # contracted-mode sharding over RCCL (also declared in include/ctc_tc.h)
 SHARDED_SYMBOLS = (
@@ -31,7 +33,9 @@ SQ_CHUNK_OFF_A, SQ_CHUNK_OFF_B, SQ_CHUNK_OFF_PARTIAL, SQ_CHUNK_OFF_OUT, SQ_CHUNK
 # every symbol include/ctc_fastr.h declares
 FASTR_SYMBOLS = ("ctc_fastr_best_offsets", "ctc_fastr_sw_align", "ctc_fastr_sw_workspace_bytes")
 
-F64, F32, BF16 = 0, 1, 2
+F64, F32, BF16, F8E4M3, F8E5M2 = 0, 1, 2, 3, 4
+BLOCK_ROWS, BLOCK_TILES = 0, 1
+GROUPS_ROWS, GROUPS_CONTRACTED = 0, 1
 
 # ctc_tc_query
 Q_NAMES, Q_CLASSES, Q_EXTENTS = 0, 1, 2
@@ -43,6 +47,13 @@ Q_ROW_A, Q_K_A, Q_K_B, Q_COL_B, Q_ROW_C, Q_COL_C, Q_BAT_A, Q_BAT_B, Q_BAT_C = ra
 Q_FLOPS = 26
 Q_SCHEDULE = 27
 Q_SPANS = 28
+
+
+class ScaledMatrix(ctypes.Structure):
+    """ctc_tc_scaled_matrix"""
+    _fields_ = [("q", ctypes.c_void_p), ("ld", ctypes.c_int64), ("batch_stride", ctypes.c_int64), ("scale", ctypes.c_void_p),
+                ("scale_row", ctypes.c_int64), ("scale_block", ctypes.c_int64), ("scale_batch", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("block", ctypes.c_int32)]
 
 
 class CtcError(RuntimeError):
@@ -104,6 +115,19 @@ def load():
     L.ctc_tc_fill.argtypes = [vp, ctypes.c_int64, ctypes.c_uint64, ctypes.c_int64, ctypes.c_int, vp]
     L.ctc_tc_grouped_contract.restype = ctypes.c_int
     L.ctc_tc_grouped_contract.argtypes = [vp, ctypes.c_int, ctypes.c_int, ctypes.c_double, vp, vp, ctypes.c_double, vp, vp]
+    i64, f64, smp = ctypes.c_int64, ctypes.c_double, ctypes.POINTER(ScaledMatrix)
+    L.ctc_tc_block_quantize.restype = ctypes.c_int
+    L.ctc_tc_block_quantize.argtypes = [vp, i64, i64, i64, i64, i64, ctypes.c_int, smp, smp, vp]
+    L.ctc_tc_scaled_workspace_bytes.restype = i64
+    L.ctc_tc_scaled_workspace_bytes.argtypes = [i64, i64, i64, i64]
+    L.ctc_tc_scaled_contract.restype = ctypes.c_int
+    L.ctc_tc_scaled_contract.argtypes = [i64, i64, i64, i64, smp, smp, f64, f64, vp, i64, i64, ctypes.c_int, vp, i64, vp]
+    L.ctc_tc_scaled_grouped_contract.restype = ctypes.c_int
+    L.ctc_tc_scaled_grouped_contract.argtypes = [ctypes.c_int, i64, vp, i64, i64, i64, smp, smp, f64, f64, vp, i64, i64, ctypes.c_int, vp]
+    L.ctc_tc_expert_workspace_bytes.restype = i64
+    L.ctc_tc_expert_workspace_bytes.argtypes = [i64, i64, i64]
+    L.ctc_tc_expert_layer.restype = ctypes.c_int
+    L.ctc_tc_expert_layer.argtypes = [i64, i64, i64, i64, i64, vp, i64, smp, smp, vp, i64, vp, i64, vp, i64, vp, i64, vp]
     L.ctc_tc_time_execute.restype = ctypes.c_int
     L.ctc_tc_time_execute.argtypes = [vp, ctypes.c_double, vp, vp, ctypes.c_double, vp, vp,
                                       ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_double)]

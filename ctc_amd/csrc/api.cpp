@@ -786,6 +786,8 @@ int64_t ctc_tc_get_option(const char *name)
     if (n == "launches_classic") return g_launches_classic.load();
     if (n == "launches_stream") return g_launches_stream.load();
     if (n == "launches_stream_f64_dma") return g_launches_stream_dma.load();
+    const int64_t scaled = ctc_internal::scaled_counter(name);
+    if (scaled >= 0) return scaled;
     return fail(CTC_TC_EINVAL, "unknown option '" + n + "'");
 }
 

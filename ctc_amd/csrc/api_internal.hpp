@@ -43,6 +43,9 @@ struct DeviceTables {
 int set_last_error(int code, const std::string &msg);
 int set_last_hip_error(hipError_t e, const char *what);
 
+// launches of the block-scaled products by kernel (scaled_api.cpp); -1: no such counter
+int64_t scaled_counter(const char *name);
+
 // No C++ exception leaves the C ABI: the body of an entry point that allocates host memory (plans, offset
 // tables, strings) stands between these two.
 #define CTC_ABI_TRY try {

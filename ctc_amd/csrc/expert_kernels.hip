@@ -1,0 +1,301 @@
+// A whole mixture-of-experts layer for a few tokens on gfx950, in two kernels:
+//   y[t] = sum_j gate[t, j] * D_e ( silu(G_e x_t) * (U_e x_t) ),  e = pick[t, j],
+// weights in e4m3 with one f32 scale per 128 x 128 tile ([G_e; U_e] is one matrix of 2 * inner rows), x and y in bf16.
+//
+// All there is to read is the picked experts' weights, each once: HBM (or, for one token, latency) bounds both kernels.
+// The matrix core multiplies in bf16: e4m3 codes are exact in bf16 and x is bf16 already, so nothing is rounded on the way in;
+// sums are f32 and a block of 128 is scaled in f32 before it is added.  The tokens of an expert are the MFMA's columns,
+// packed from the router's picks by one ballot (lane = token): a token that did not pick the expert is in no column, so
+// that nothing an expert's weights hold (NaN among it) reaches a token that did not pick it.
+// Between the kernels h = gate * silu(G x) * (U x) is rounded to bf16, as an activation between two layers is: the second
+// kernel's MFMA takes 16 bits, and every workgroup reads the whole h, half the bytes of f32.
+#include "scaled_device.hpp"
+
+namespace ctc {
+
+using namespace scaled;
+
+namespace {
+
+constexpr int kWaves = 8;
+static_assert(kExpertMaxTokens == 64, "a token is a lane of a wave");
+static_assert(kExpertMaxExperts / 32 == 128, "a lane of the listing wave reads two words of the experts' bits");
+
+// one block of 128 contracted elements of a row, as a lane of group fg holds it: bytes k .. k + 16 and k + 64 .. k + 80
+struct Codes {
+    uint4 lo, hi;
+};
+__device__ __forceinline__ Codes load_codes(const uint8_t *row, int64_t k, int64_t k_end, bool whole)
+{
+    Codes c;
+    if (whole) {
+        __builtin_memcpy(&c.lo, row + k, 16);
+        __builtin_memcpy(&c.hi, row + k + 64, 16);
+    } else {
+        c.lo = load_chunk(row, k, k_end);
+        c.hi = load_chunk(row, k + 64, k_end);
+    }
+    return c;
+}
+// the bf16 elements at the same places
+struct Halves {
+    uint4 v[4];
+};
+__device__ __forceinline__ Halves load_halves(const uint8_t *row, int64_t k, int64_t k_end, bool whole)
+{
+    Halves h;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int64_t at = 2 * (k + (q & 1) * 8 + (q >> 1) * 64);
+        if (whole) __builtin_memcpy(&h.v[q], row + at, 16);
+        else h.v[q] = load_chunk(row, at, 2 * k_end);
+    }
+    return h;
+}
+__device__ __forceinline__ v4f block_product(const Codes &c, const Halves &h)
+{
+    v4f d = {0.f, 0.f, 0.f, 0.f};
+    const uint32_t w[8] = {c.lo.x, c.lo.y, c.lo.z, c.lo.w, c.hi.x, c.hi.y, c.hi.z, c.hi.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen<0>(w[2 * q], w[2 * q + 1]), __builtin_bit_cast(bf16x8, h.v[q]), d, 0, 0, 0);
+    return d;
+}
+
+// the picks of one token, held by the token's lane; -1 beyond `top` and for lanes beyond the tokens
+struct Picks {
+    int e[kExpertMaxTop];
+};
+__device__ __forceinline__ Picks load_picks(const ExpertParams &p, int lane)
+{
+    Picks k;
+#pragma unroll
+    for (int j = 0; j < kExpertMaxTop; ++j) k.e[j] = j < p.top && lane < p.tokens ? p.pick[lane * p.ld_pick + j] : -1;
+    return k;
+}
+// the first place of `e` among the token's picks, -1: none
+__device__ __forceinline__ int place_of(const Picks &k, int e)
+{
+    int at = -1;
+#pragma unroll
+    for (int j = kExpertMaxTop - 1; j >= 0; --j)
+        if (k.e[j] == e) at = j;
+    return at;
+}
+
+// h = gate * silu(G x) * (U x) for 16 of an expert's inner rows and all its tokens.  Workgroup (slice, y): y is a pair
+// (token, place) where there are fewer pairs than experts, and only the first pair of an expert works; else y is the expert.
+// Eight waves share the contracted blocks; their partial sums meet in LDS, in wave order.
+template <bool UNI> __global__ void __launch_bounds__(kWaves * 64) expert_up_kernel(ExpertParams p, int by_pair)
+{
+    __shared__ __attribute__((aligned(16))) float part[kWaves][2][256];
+    __shared__ int token_of[64], row_of[64];
+    __shared__ float gate_of[64];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int fr = lane & 15, fg = lane >> 4;
+    const int64_t i0 = (int64_t)blockIdx.x * 16;
+    int e = blockIdx.y;
+    if (by_pair) e = p.pick[(blockIdx.y / p.top) * p.ld_pick + blockIdx.y % p.top];
+    e = __builtin_amdgcn_readfirstlane(e);
+    if (e < 0 || e >= p.experts) return;
+    const Picks picks = load_picks(p, lane);
+    const int place = place_of(picks, e);
+    const unsigned long long mask = __ballot(place >= 0);
+    if (mask == 0) return;
+    if (by_pair) {  // the expert's first pair: the first token's first place
+        const int first = __ffsll((long long)mask) - 1;
+        if ((unsigned)(first * p.top + __shfl(place, first)) != blockIdx.y) return;
+    }
+    const int count = __popcll(mask);
+    if (wave == 0 && place >= 0) {
+        float g = 0.f;  // a token may name an expert twice: its weights add
+#pragma unroll
+        for (int j = 0; j < kExpertMaxTop; ++j)
+            if (picks.e[j] == e) g += p.gate[lane * p.ld_gate + j];
+        const int c = __popcll(mask & ((1ull << lane) - 1));
+        token_of[c] = lane;
+        row_of[c] = lane * p.top + place;
+        gate_of[c] = g;
+    }
+    __syncthreads();
+
+    const int64_t iu = i0 + fr < p.inner ? i0 + fr : p.inner - 1;
+    const uint8_t *w_gate = p.up.q + e * p.up.batch + iu * p.up.ld, *w_up = w_gate + p.inner * p.up.ld;
+    const float *S = p.up.scale + e * p.up.s_batch;
+    const float *s_gate[UNI ? 1 : 4], *s_up[UNI ? 1 : 4];
+#pragma unroll
+    for (int r = 0; r < (UNI ? 1 : 4); ++r) {
+        int64_t i = UNI ? i0 : i0 + fg * 4 + r;
+        i = i < p.inner ? i : p.inner - 1;
+        s_gate[r] = S + (i >> 7) * p.up.s_row;
+        s_up[r] = S + ((p.inner + i) >> 7) * p.up.s_row;
+    }
+    const int steps = (int)((p.hidden + kScaleBlock - 1) / kScaleBlock);
+    for (int c0 = 0; c0 < count; c0 += 16) {
+        const int c = c0 + fr < count ? c0 + fr : count - 1;
+        const uint8_t *x = static_cast<const uint8_t *>(p.x) + 2 * token_of[c] * p.ldx;
+        v4f ag = {0.f, 0.f, 0.f, 0.f}, au = {0.f, 0.f, 0.f, 0.f};
+        constexpr int U = 2;
+        for (int s0 = wave; s0 < steps; s0 += kWaves * U) {
+            Codes cg[U], cu[U];
+            Halves h[U];
+            float fgate[U][UNI ? 1 : 4], fup[U][UNI ? 1 : 4];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int s = s0 + u * kWaves;
+                if (s >= steps) break;
+                const int64_t k = (int64_t)s * kScaleBlock + fg * 16;
+                const bool whole = (int64_t)(s + 1) * kScaleBlock <= p.hidden;
+                cg[u] = load_codes(w_gate, k, p.hidden, whole);
+                cu[u] = load_codes(w_up, k, p.hidden, whole);
+                h[u] = load_halves(x, k, p.hidden, whole);
+#pragma unroll
+                for (int r = 0; r < (UNI ? 1 : 4); ++r) {
+                    fgate[u][r] = s_gate[r][s * p.up.s_blk];
+                    fup[u][r] = s_up[r][s * p.up.s_blk];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (s0 + u * kWaves >= steps) break;
+                const v4f dg = block_product(cg[u], h[u]), du = block_product(cu[u], h[u]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    ag[r] = __builtin_fmaf(dg[r], fgate[u][UNI ? 0 : r], ag[r]);
+                    au[r] = __builtin_fmaf(du[r], fup[u][UNI ? 0 : r], au[r]);
+                }
+            }
+        }
+        *reinterpret_cast<v4f *>(&part[wave][0][fr * 16 + fg * 4]) = ag;
+        *reinterpret_cast<v4f *>(&part[wave][1][fr * 16 + fg * 4]) = au;
+        __syncthreads();
+        if (t < 256) {  // (column, row)
+            const int col = c0 + (t >> 4), row = t & 15;
+            float g = 0.f, u = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                g += part[w][0][t];
+                u += part[w][1][t];
+            }
+            if (col < count && i0 + row < p.inner) {
+                const float h = g / (1.f + expf(-g)) * u * gate_of[col];
+                static_cast<uint16_t *>(p.h)[row_of[col] * p.inner + i0 + row] = to_bf16(h);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// y for 16 of the hidden rows and all tokens: the waves share the picked experts (several waves an expert's contracted
+// blocks where there are few), add an expert's columns to their own LDS copy of the 16 x tokens result, and the
+// copies are summed in wave order: no atomics on values, the same bits on every run.
+__global__ void __launch_bounds__(kWaves * 64) expert_down_kernel(ExpertParams p, int k_parts)
+{
+    extern __shared__ __attribute__((aligned(16))) float y_part[];  // [wave][token][16]
+    __shared__ uint32_t bits[kExpertMaxExperts / 32];
+    __shared__ int list[kExpertMaxPairs];
+    __shared__ int listed;
+    __shared__ int columns[kWaves][64];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int fr = lane & 15, fg = lane >> 4;
+    const int64_t r0 = (int64_t)blockIdx.x * 16;
+    const int per_wave = p.tokens * 16;
+    for (int i = t; i < kWaves * per_wave; i += kWaves * 64) y_part[i] = 0.f;
+    if (t < kExpertMaxExperts / 32) bits[t] = 0;
+    __syncthreads();
+    for (int i = t; i < p.tokens * p.top; i += kWaves * 64) {
+        const int e = p.pick[(i / p.top) * p.ld_pick + i % p.top];
+        if (e >= 0 && e < p.experts) atomicOr(&bits[e >> 5], 1u << (e & 31));
+    }
+    __syncthreads();
+    if (wave == 0) {  // the experts in ascending order
+        const uint32_t w0 = bits[2 * lane], w1 = bits[2 * lane + 1];
+        const int n = __popc(w0) + __popc(w1);
+        int sum = n;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(sum, d);
+            if (lane >= d) sum += o;
+        }
+        int at = sum - n;
+        for (uint32_t b = w0; b; b &= b - 1) list[at++] = 64 * lane + __ffs((int)b) - 1;
+        for (uint32_t b = w1; b; b &= b - 1) list[at++] = 64 * lane + 32 + __ffs((int)b) - 1;
+        if (lane == 63) listed = sum;
+    }
+    const Picks picks = load_picks(p, lane);
+    __syncthreads();
+    const int experts = listed, lanes = kWaves / k_parts;
+    const int part = wave / lanes, steps = (int)((p.inner + kScaleBlock - 1) / kScaleBlock);
+    const int64_t row = r0 + fr < p.hidden ? r0 + fr : p.hidden - 1;
+    float *mine = y_part + wave * per_wave;
+    for (int u = wave % lanes; u < experts; u += lanes) {
+        const int e = __builtin_amdgcn_readfirstlane(list[u]);
+        const int place = place_of(picks, e);
+        const unsigned long long mask = __ballot(place >= 0);
+        const int count = __popcll(mask);
+        if (place >= 0) columns[wave][__popcll(mask & ((1ull << lane) - 1))] = lane * p.top + place;
+        __builtin_amdgcn_wave_barrier();  // one wave's LDS accesses are in order
+        const uint8_t *w = p.down.q + e * p.down.batch + row * p.down.ld;
+        const float *S = p.down.scale + e * p.down.s_batch + (r0 >> 7) * p.down.s_row;
+        for (int c0 = 0; c0 < count; c0 += 16) {
+            const int pair = columns[wave][c0 + fr < count ? c0 + fr : count - 1];
+            const uint8_t *h = static_cast<const uint8_t *>(p.h) + 2 * pair * p.inner;
+            v4f acc = {0.f, 0.f, 0.f, 0.f};
+            constexpr int U = 4;
+            for (int s0 = part; s0 < steps; s0 += k_parts * U) {
+                Codes c[U];
+                Halves v[U];
+                float f[U];
+#pragma unroll
+                for (int q = 0; q < U; ++q) {
+                    const int s = s0 + q * k_parts;
+                    if (s >= steps) break;
+                    const int64_t k = (int64_t)s * kScaleBlock + fg * 16;
+                    const bool whole = (int64_t)(s + 1) * kScaleBlock <= p.inner;
+                    c[q] = load_codes(w, k, p.inner, whole);
+                    v[q] = load_halves(h, k, p.inner, whole);
+                    f[q] = S[s * p.down.s_blk];
+                }
+#pragma unroll
+                for (int q = 0; q < U; ++q) {
+                    if (s0 + q * k_parts >= steps) break;
+                    const v4f d = block_product(c[q], v[q]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(d[r], f[q], acc[r]);
+                }
+            }
+            if (c0 + fr < count) {
+                v4f *dst = reinterpret_cast<v4f *>(mine + (pair / p.top) * 16 + fg * 4);
+                *dst += acc;
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    for (int i = t; i < per_wave; i += kWaves * 64) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) v += y_part[w * per_wave + i];
+        const int64_t r = r0 + (i & 15);
+        if (r < p.hidden) static_cast<uint16_t *>(p.y)[(i >> 4) * p.ldy + r] = to_bf16(v);
+    }
+}
+
+}  // namespace
+
+hipError_t launch_expert_layer(const ExpertParams &p, hipStream_t stream)
+{
+    const int pairs = p.tokens * p.top;
+    const int by_pair = pairs < p.experts;
+    const dim3 up((unsigned)((p.inner + 15) / 16), (unsigned)(by_pair ? pairs : p.experts));
+    if (p.inner % 16 == 0) hipLaunchKernelGGL((expert_up_kernel<true>), up, dim3(kWaves * 64), 0, stream, p, by_pair);
+    else hipLaunchKernelGGL((expert_up_kernel<false>), up, dim3(kWaves * 64), 0, stream, p, by_pair);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    // at most `pairs` experts: with fewer than eight, several waves share one expert's contracted blocks
+    const int k_parts = pairs >= 8 ? 1 : pairs >= 4 ? 2 : pairs >= 2 ? 4 : 8;
+    hipLaunchKernelGGL(expert_down_kernel, dim3((unsigned)((p.hidden + 15) / 16)), dim3(kWaves * 64), (size_t)kWaves * p.tokens * 16 * 4, stream, p, k_parts);
+    return hipGetLastError();
+}
+
+}  // namespace ctc

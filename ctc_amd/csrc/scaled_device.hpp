@@ -1,0 +1,124 @@
+// Device-side pieces shared by the block-scaled product kernels.
+#pragma once
+
+#include "scaled.hpp"
+
+namespace ctc {
+namespace scaled {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// eight 8-bit codes (FMT 0 e4m3, 1 e5m2) to bf16, exactly
+template <int FMT> __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi)
+{
+    bf16x2 a, b, c, d;
+    if constexpr (FMT) {
+        a = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, 1.f, true);
+        c = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, 1.f, true);
+    } else {
+        a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true);
+        c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true);
+    }
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// A lane's 32 codes of a block of 128 as an operand of the matrix core.  FAST: the codes themselves, for one
+// v_mfma_f32_16x16x128_f8f6f4.  That is four times the rate of the bf16 form, but the 8-bit forms of the matrix core (the
+// 16x16x32 ones too) align the products of each group of eight k to the largest one and drop what lies below its 2^-13 (measured:
+// 2^16 + 2^3 in one group is exact, 2^16 + 2^2 gives 2^16; between groups the sum is f32).  On normal operands that is
+// 1.5e-5 of the result's norm: far below the 2^-9 of a bf16 result, far above the 2^-24 of an f32 one.  Otherwise: the codes
+// widened to bf16 (exactly) for four v_mfma_f32_16x16x32_bf16, which sum in f32.
+template <int FMT, bool FAST> struct BlockOperand;
+template <int FMT> struct BlockOperand<FMT, true> {
+    v8i v;
+    __device__ __forceinline__ void set(const v4i &lo, const v4i &hi) { v = v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}; }
+};
+template <int FMT> struct BlockOperand<FMT, false> {
+    bf16x8 v[4];
+    __device__ __forceinline__ void set(const v4i &lo, const v4i &hi)
+    {
+        v[0] = widen<FMT>(lo[0], lo[1]);
+        v[1] = widen<FMT>(lo[2], lo[3]);
+        v[2] = widen<FMT>(hi[0], hi[1]);
+        v[3] = widen<FMT>(hi[2], hi[3]);
+    }
+};
+// the 16 x 16 sums of a block's products (rows of B x rows of A)
+template <int FA, bool FAST> __device__ __forceinline__ v4f block_sums(const BlockOperand<0, FAST> &b, const BlockOperand<FA, FAST> &a)
+{
+    v4f d = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (FAST) {
+        d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.v, a.v, d, 0, FA, 0, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.v[q], a.v[q], d, 0, 0, 0);
+    }
+    return d;
+}
+
+// 16 bytes of a row from byte k on, zeros from byte k_end on; any alignment
+__device__ __forceinline__ uint4 load_chunk(const uint8_t *row, int64_t k, int64_t k_end)
+{
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if (k + 16 <= k_end) {
+        __builtin_memcpy(&u, row + k, 16);
+    } else if (k < k_end) {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (k + i < k_end) w[i >> 2] |= (uint32_t)row[k + i] << (8 * (i & 3));
+        u = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return u;
+}
+
+__device__ __forceinline__ int64_t clamp_offset(int64_t o, int64_t hi) { return o < 0 ? 0 : (o > hi ? hi : o); }
+
+
+__device__ __forceinline__ uint16_t to_bf16(float f)
+{
+    const uint32_t u = __float_as_uint(f);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40);  // NaN stays one
+    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1)) >> 16);
+}
+__device__ __forceinline__ float from_bf16(uint16_t h) { return __uint_as_float((uint32_t)h << 16); }
+
+// four consecutive n of row m, alpha and beta applied in f32, rounded once
+__device__ __forceinline__ void store4(const ScaledGemmParams &p, int64_t at, int64_t n, v4f v, bool vec)
+{
+    if (p.c_f32) {
+        float *c = static_cast<float *>(p.C) + at;
+        if (vec && n + 4 <= p.N) {
+            v4f o = v * p.alpha;
+            if (p.beta != 0.f) o += p.beta * *reinterpret_cast<const v4f *>(c);
+            *reinterpret_cast<v4f *>(c) = o;
+            return;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (n + r < p.N) c[r] = p.alpha * v[r] + (p.beta != 0.f ? p.beta * c[r] : 0.f);
+        return;
+    }
+    uint16_t *c = static_cast<uint16_t *>(p.C) + at;
+    if (vec && n + 4 <= p.N) {
+        uint2 old = make_uint2(0, 0);
+        if (p.beta != 0.f) old = *reinterpret_cast<const uint2 *>(c);
+        const uint16_t h[4] = {(uint16_t)old.x, (uint16_t)(old.x >> 16), (uint16_t)old.y, (uint16_t)(old.y >> 16)};
+        uint16_t o[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = to_bf16(p.alpha * v[r] + (p.beta != 0.f ? p.beta * from_bf16(h[r]) : 0.f));
+        *reinterpret_cast<uint2 *>(c) = make_uint2((uint32_t)o[0] | (uint32_t)o[1] << 16, (uint32_t)o[2] | (uint32_t)o[3] << 16);
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (n + r < p.N) c[r] = to_bf16(p.alpha * v[r] + (p.beta != 0.f ? p.beta * from_bf16(c[r]) : 0.f));
+}
+
+}  // namespace scaled
+}  // namespace ctc

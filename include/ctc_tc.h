@@ -38,7 +38,8 @@ extern "C" {
 
 typedef struct ctc_tc_plan ctc_tc_plan;
 
-enum ctc_tc_dtype { CTC_TC_F64 = 0, CTC_TC_F32 = 1, CTC_TC_BF16 = 2 };
+/* the 8-bit types (OCP e4m3 without infinities, OCP e5m2) belong to the block-scaled operators alone */
+enum ctc_tc_dtype { CTC_TC_F64 = 0, CTC_TC_F32 = 1, CTC_TC_BF16 = 2, CTC_TC_F8E4M3 = 3, CTC_TC_F8E5M2 = 4 };
 
 enum ctc_tc_status {
     CTC_TC_OK = 0,
@@ -172,6 +173,8 @@ int ctc_tc_set_option(const char *name, int64_t value);
  * register-staged), "launches_stream_f64_dma", "launches_bf16_ring" (the bf16 256-tile ring kernel, a
  * subset of "launches_classic"), "padded_executions" (executions that went through the padded copies; their GEMM
  * counts in the launch counters as well), "launches_grouped" (batched plans that took the grouped kernel).
+ * "launches_scaled_skinny" / "launches_scaled_128" / "launches_scaled_256": block-scaled products by kernel;
+ * "launches_scaled_split": those among them whose contracted index was split.
  * Negative ctc_tc_status for an unknown name. */
 int64_t ctc_tc_get_option(const char *name);
 
@@ -366,6 +369,92 @@ typedef struct ctc_tc_small_gemm {
 
 int ctc_tc_grouped_contract(const ctc_tc_small_gemm *problems, int count, int dtype, double alpha,
                             const void *A, const void *B, double beta, void *C, void *stream);
+
+/*
+ * ---- Block-scaled 8-bit operators (linear layers and experts, training and serving) --------------------------------
+ * No reference counterpart.  A matrix of 8-bit codes stands for q(r, c) * scale, with one f32 scale for every 128
+ * consecutive columns of a row (CTC_TC_BLOCK_ROWS: scale(r, c / 128)) or for every 128 x 128 tile (CTC_TC_BLOCK_TILES:
+ * scale(r / 128, c / 128)); the last block of a row or column may be partly filled.  Columns are the CONTRACTED index
+ * of the products, so a matrix that is contracted along its rows as well (a weight in a backward pass, activations in a
+ * weight's gradient) is needed transposed too: the quantiser writes both from one reading.
+ *
+ * Codes have unit stride along a row and any leading dimension; pointers and strides may have any alignment (with
+ * q, ld and batch_stride at multiples of 16 the large products run on LDS-DMA, otherwise through registers).
+ * The scales' strides are free; the quantiser's callers usually keep the row index fastest (scale_row = 1), which is
+ * how the products read them.  No entry point below allocates or synchronises: all may be captured in a HIP graph, and
+ * calls on different streams may overlap unless they share a result or a workspace.  Results must not overlap operands.
+ */
+enum ctc_tc_block { CTC_TC_BLOCK_ROWS = 0, CTC_TC_BLOCK_TILES = 1 };
+
+typedef struct ctc_tc_scaled_matrix {
+    void *q;                 /* device: 8-bit codes */
+    int64_t ld, batch_stride;
+    float *scale;            /* device */
+    int64_t scale_row;       /* stride of a row (BLOCK_ROWS) or of a tile of 128 rows */
+    int64_t scale_block;     /* stride of a block of 128 columns */
+    int64_t scale_batch;
+    int32_t dtype;           /* CTC_TC_F8E4M3 or CTC_TC_F8E5M2 */
+    int32_t block;           /* ctc_tc_block */
+} ctc_tc_scaled_matrix;
+
+/*
+ * Quantises x (rows x cols, f32 or bf16, unit column stride; `batch` matrices) into `out` (rows x cols) and / or `out_t`
+ * (cols x rows, the transpose, with its own blocks along the rows of x); either may be NULL, both have one dtype and block kind.
+ *   top   = max(2^-100, largest finite |x| of the block)
+ *   scale = top / L,  q = round-to-nearest-even to 8 bits of (x * (L / top)),  L = 448 (e4m3) or 57344 (e5m2),
+ * in f32.  Infinities turn into NaN (e4m3) or infinity (e5m2) and NaN into NaN; they do not enter `top`.
+ */
+int ctc_tc_block_quantize(const void *x, int64_t rows, int64_t cols, int64_t ldx, int64_t batch, int64_t batch_stride_x, int src_dtype,
+                          const ctc_tc_scaled_matrix *out, const ctc_tc_scaled_matrix *out_t, void *stream);
+
+/*
+ * C(m, n) = alpha * sum_k A(m, k) B(n, k) + beta * C(m, n) of block-scaled operands, `batch` products.  The codes' products
+ * are summed inside a block of 128 and scaled and summed in f32 over the blocks; alpha and beta apply in f32 and the
+ * result is rounded once.  The sums inside a block are f32 where C is f32 or m is at most 32; for a larger product with a bf16 C
+ * they are those of the matrix core's 8-bit form, which drops from each product what lies below 2^-13 of the largest one
+ * among eight neighbours (1.5e-5 of the result's norm on normal operands, 1/130 of the bf16 rounding).  A is e4m3 or e5m2, B e4m3, either with row or tile scales; C is f32 or bf16 with unit
+ * column stride.  beta == 0 does not read C.  k == 0 leaves beta * C.
+ *   a linear layer y = x W^T:  A = x (rows), B = W (tiles);
+ *   its gradients:             dx: A = dy (rows), B = the transposed tiles of W;
+ *                              dW: A = the transpose of dy (rows), B = the transpose of x (rows).
+ * workspace: NULL, or ctc_tc_scaled_workspace_bytes(m, n, k, batch) bytes (16-byte aligned) that let a product of few
+ * tiles split a long contracted index over more workgroups (partial sums are added in a fixed order).  With a smaller
+ * workspace the split is smaller.  The contents need not be kept or cleared between calls.
+ */
+int64_t ctc_tc_scaled_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t batch);
+int ctc_tc_scaled_contract(int64_t m, int64_t n, int64_t k, int64_t batch, const ctc_tc_scaled_matrix *a, const ctc_tc_scaled_matrix *b,
+                           double alpha, double beta, void *C, int64_t ldc, int64_t batch_stride_c, int c_dtype, void *workspace,
+                           int64_t workspace_bytes, void *stream);
+
+/*
+ * The same over ragged groups (experts) in one launch.  `offsets` is a DEVICE array of groups + 1 ascending values:
+ *   CTC_TC_GROUPS_ROWS        group g owns rows [offsets[g], offsets[g + 1]) of A (m x k) and C (m x n) and multiplies them by
+ *                             its own B (n x k at batch_stride * g).  Rows of C outside every group are not written.
+ *   CTC_TC_GROUPS_CONTRACTED  group g owns that range of the contracted index of A (m x k) and B (n x k) and writes its
+ *                             own C (m x n at group_stride_c * g); an empty group writes beta * C.  Offsets are multiples
+ *                             of 128 or k itself (others are taken at the block they fall into: a block has one scale).
+ * The offsets stay on the device, so nothing can check them in front of the launch: values outside the operands are taken as
+ * the nearer end and a group that would end before it starts as empty, so no access leaves the operands; where groups
+ * overlap, results are undefined.
+ */
+enum ctc_tc_groups { CTC_TC_GROUPS_ROWS = 0, CTC_TC_GROUPS_CONTRACTED = 1 };
+int ctc_tc_scaled_grouped_contract(int along, int64_t groups, const int32_t *offsets, int64_t m, int64_t n, int64_t k,
+                                   const ctc_tc_scaled_matrix *a, const ctc_tc_scaled_matrix *b, double alpha, double beta, void *C,
+                                   int64_t ldc, int64_t group_stride_c, int c_dtype, void *stream);
+
+/*
+ * A mixture-of-experts layer for a few tokens (at most 64, 16 experts each, 4096 experts in all), in two launches:
+ *   y(t) = sum_j gate(t, j) * D_e (silu(G_e x(t)) * (U_e x(t))),  e = pick(t, j),
+ * x and y bf16, `up` the e4m3 matrices [G_e; U_e] (2 inner x hidden), `down` the D_e (hidden x inner), both with
+ * CTC_TC_BLOCK_TILES and batch_stride from expert to expert.  pick and gate are DEVICE arrays (tokens x top).  A pick
+ * outside [0, experts) contributes nothing; an expert picked twice by a token counts with the sum of its gates.  The
+ * weights of experts that nobody picks are not read.  gate * silu(G x) * (U x) is rounded to bf16 between the launches;
+ * all sums are f32, in a fixed order.  workspace: ctc_tc_expert_workspace_bytes(tokens, top, inner) bytes.
+ */
+int64_t ctc_tc_expert_workspace_bytes(int64_t tokens, int64_t top, int64_t inner);
+int ctc_tc_expert_layer(int64_t tokens, int64_t top, int64_t experts, int64_t hidden, int64_t inner, const void *x, int64_t ldx,
+                        const ctc_tc_scaled_matrix *up, const ctc_tc_scaled_matrix *down, const int32_t *pick, int64_t ld_pick,
+                        const float *gate, int64_t ld_gate, void *y, int64_t ldy, void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
  * Synthetic operand generator on the device: element k (packed order) =
