@@ -16,8 +16,6 @@ using namespace scaled;
 
 namespace {
 
-__device__ __attribute__((aligned(16))) const uint8_t zero_chunk[16] = {};
-
 // What a workgroup multiplies: rows [m0, m_end) x columns [n0, N) over the contracted [k_begin, k_end), written to C
 struct Item {
     int64_t m0, m_end, n0, k_begin, k_end;
@@ -88,6 +86,13 @@ __device__ __forceinline__ void grouped_order(int64_t id, int64_t nbm, int64_t n
     tn = in / h;
 }
 
+// a value that is the same in all lanes, into scalar registers
+__device__ __forceinline__ int64_t uniform(int64_t v)
+{
+    const int lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+    return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+}
+
 template <int BM, int BN> __device__ __forceinline__ bool find_item(const ScaledGemmParams &p, Item &it)
 {
     int64_t id = blockIdx.x, tm, tn;
@@ -101,11 +106,8 @@ template <int BM, int BN> __device__ __forceinline__ bool find_item(const Scaled
         grouped_order(xcd_run(id, total), rows, p.nbn, tm, tn);
         int g = 0;
         if (!find_group_tile(p.offsets, p.batch, p.M, BM, tm, g, it.m0, it.m_end)) return false;
-        // one value for the whole workgroup: kept in scalar registers
-        it.entry = __builtin_amdgcn_readfirstlane(g);
-        it.m0 = __builtin_amdgcn_readfirstlane((int)it.m0);
-        it.m_end = __builtin_amdgcn_readfirstlane((int)it.m_end);
-        it.n0 = (int64_t)__builtin_amdgcn_readfirstlane((int)tn) * BN;
+        it.entry = g;
+        it.n0 = tn * BN;
         return true;
     }
     const int64_t per_entry = (int64_t)p.nbm * p.nbn, total = per_entry * p.batch * p.split;
@@ -133,15 +135,30 @@ template <int BM, int BN> __device__ __forceinline__ bool find_item(const Scaled
     return true;
 }
 
-// BM x BN tile, WM x WN waves.  FA: A holds e5m2.  BUNI: B's scale is one per 128 x 128 tile, hence uniform in a wave.
-// DMA: both operands 16-byte aligned with row pitches that are multiples of 16: their blocks go global -> LDS by DMA;
-// otherwise every chunk passes through registers (byte-exact at any alignment).
+__device__ __forceinline__ void store_partial(float *w, int64_t left, v4f v, bool vec)
+{
+    if (vec) {
+        *reinterpret_cast<v4f *>(w) = v;
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (r < left) w[r] = v[r];
+}
+
+// BM x BN tile, WM x WN waves.  FA: A holds e5m2.  FAST: see BlockOperand.  BUNI: B's scale is one per 128 x 128 tile, hence
+// uniform in a wave.  DMA: both operands 16-byte aligned with row pitches that are multiples of 16: their blocks go
+// global -> LDS by DMA; otherwise every chunk passes through registers (byte-exact at any alignment).
 //
 // LDS, two stages of a block each: rows of 128 bytes, 16-byte chunk c of row r at c ^ (r / 2 & 7).  A fragment is the
 // chunks g and g + 4 of row l % 16 (g = l / 16), for both operands alike, so that the k order inside the MFMA's block
 // does not matter; with the XOR sixteen lanes that ds_read_b128 serves together fall on sixteen different 16-byte slots.
+//
+// A wave walks its row tiles with one tile's results in hand while the next one's MFMAs run: fragment i + 1 is
+// requested, tile i multiplied, tile i - 1 scaled and added.  The order is pinned (sched_barrier): left alone, the
+// compiler requests every fragment first and spills.
 template <int FA, bool FAST, bool BUNI, int BM, int BN, int WM, int WN, bool DMA>
-__global__ void __launch_bounds__(WM *WN * 64) scaled_gemm_kernel(ScaledGemmParams p)
+__global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmParams p)
 {
     constexpr int T = WM * WN * 64;
     constexpr int WTM = BM / WM, WTN = BN / WN, MT = WTM / 16, NT = WTN / 16;
@@ -149,102 +166,102 @@ __global__ void __launch_bounds__(WM *WN * 64) scaled_gemm_kernel(ScaledGemmPara
     constexpr int NA = BM * 8 / T, NB = BN * 8 / T;  // chunks a thread stages
     static_assert(BM * 8 % T == 0 && BN * 8 % T == 0 && (!BUNI || (128 % WTN == 0 && BN % WTN == 0)), "tile");
     static_assert(T / 8 % 16 == 0, "a thread's rows are 16 or more apart: one swizzle term for all of them");
-    __shared__ __attribute__((aligned(16))) uint8_t image[2][STAGE];
-    __shared__ __attribute__((aligned(16))) float scales[2][BM + BN];
+    static_assert(T == BM + BN && BM % 64 == 0, "a thread loads one scale a step, a wave those of one operand");
+    __shared__ __attribute__((aligned(16))) uint8_t image[2 * STAGE];
+    __shared__ __attribute__((aligned(16))) float scales[2 * (BM + BN)];
 
     Item it;
     if (!find_item<BM, BN>(p, it)) return;
+    it.m0 = uniform(it.m0);
+    it.m_end = uniform(it.m_end);
+    it.n0 = uniform(it.n0);
+    it.k_begin = uniform(it.k_begin);
+    it.k_end = uniform(it.k_end);
+    it.entry = uniform(it.entry);
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = wave / WN, wn = wave % WN;
     const int64_t a_entry = p.mode == kScaledDense ? it.entry : 0, b_entry = p.mode == kScaledContracted ? 0 : it.entry;
-    const uint8_t *A = p.a.q + a_entry * p.a.batch, *B = p.b.q + b_entry * p.b.batch;
-    const float *SA = p.a.scale + a_entry * p.a.s_batch, *SB = p.b.scale + b_entry * p.b.s_batch;
-
-    // staging: thread t owns chunk slot t % 8 of rows t / 8 + i * T / 8; rows beyond the operand repeat its last one
-    const int srow = t >> 3, slot = t & 7, schunk = slot ^ ((srow >> 1) & 7);
-    int64_t a_off[NA], b_off[NB];
-#pragma unroll
-    for (int i = 0; i < NA; ++i) {
-        int64_t r = it.m0 + srow + i * (T / 8);
-        a_off[i] = (r < it.m_end ? r : it.m_end - 1) * p.a.ld;
-    }
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        int64_t r = it.n0 + srow + i * (T / 8);
-        b_off[i] = (r < p.N ? r : p.N - 1) * p.b.ld;
-    }
     const int64_t steps = (it.k_end - it.k_begin + kScaleBlock - 1) / kScaleBlock;
     const int64_t blk0 = it.k_begin / kScaleBlock;
 
+    // staging: thread t owns chunk slot t % 8 of rows t / 8 + i * T / 8; rows beyond the operand repeat its last one
+    const int srow = t >> 3, slot = t & 7, schunk = slot ^ ((srow >> 1) & 7);
+    const uint8_t *A = p.a.q + a_entry * p.a.batch + it.m0 * p.a.ld + it.k_begin;
+    const uint8_t *B = p.b.q + b_entry * p.b.batch + it.n0 * p.b.ld + it.k_begin;
+    uint32_t a_off[NA], b_off[NB];  // from the tile's corner: at most 255 rows of at most 2^22 bytes where DMA is set
+    int64_t a_row[DMA ? 1 : NA], b_row[DMA ? 1 : NB];
+    const int a_last = (int)((it.m_end - it.m0 < BM ? it.m_end - it.m0 : BM) - 1), b_last = (int)((p.N - it.n0 < BN ? p.N - it.n0 : BN) - 1);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+        const int r = min(srow + i * (T / 8), a_last);
+        if constexpr (DMA) a_off[i] = (uint32_t)r * (uint32_t)p.a.ld + schunk * 16;
+        else a_row[i] = r * p.a.ld;
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int r = min(srow + i * (T / 8), b_last);
+        if constexpr (DMA) b_off[i] = (uint32_t)r * (uint32_t)p.b.ld + schunk * 16;
+        else b_row[i] = r * p.b.ld;
+    }
+    const unsigned lds0 = lds_dma::lds_addr(image) + wave * 1024;
+    const int64_t k_len = it.k_end - it.k_begin;
+
+    // stages the whole block s
     auto stage = [&](int64_t s, int buf) {
-        const int64_t k = it.k_begin + s * kScaleBlock + schunk * 16;
-        const int64_t left = it.k_end - k;
         if constexpr (DMA) {
-            const unsigned base = lds_dma::lds_addr(&image[buf][0]) + wave * 1024;
-            const bool whole = left >= 16;
+            const unsigned base = lds0 + buf * STAGE;
 #pragma unroll
-            for (int i = 0; i < NA; ++i) {
-                const void *src = whole ? A + a_off[i] + k : zero_chunk;
-                asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(base + i * (T * 16)) : "memory");
-            }
+            for (int i = 0; i < NA; ++i) lds_dma::dma16_split(A + s * kScaleBlock, a_off[i], base + i * (T * 16));
 #pragma unroll
-            for (int i = 0; i < NB; ++i) {
-                const void *src = whole ? B + b_off[i] + k : zero_chunk;
-                asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(base + BM * 128 + i * (T * 16)) : "memory");
-            }
+            for (int i = 0; i < NB; ++i) lds_dma::dma16_split(B + s * kScaleBlock, b_off[i], base + BM * 128 + i * (T * 16));
         } else {
+            const int64_t k = s * kScaleBlock + schunk * 16;
+            uint8_t *to = image + buf * STAGE + srow * 128 + slot * 16;
 #pragma unroll
-            for (int i = 0; i < NA; ++i)
-                *reinterpret_cast<uint4 *>(&image[buf][(srow + i * (T / 8)) * 128 + slot * 16]) = load_chunk(A + a_off[i], k, it.k_end);
+            for (int i = 0; i < NA; ++i) *reinterpret_cast<uint4 *>(to + i * (T * 16)) = load_chunk(A + a_row[i], k, k_len);
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
-                *reinterpret_cast<uint4 *>(&image[buf][BM * 128 + (srow + i * (T / 8)) * 128 + slot * 16]) = load_chunk(B + b_off[i], k, it.k_end);
+            for (int i = 0; i < NB; ++i) *reinterpret_cast<uint4 *>(to + BM * 128 + i * (T * 16)) = load_chunk(B + b_row[i], k, k_len);
         }
     };
-    // behind the DMA's wait: the chunk that K ends inside of, byte by byte, by the lane whose transfer wrote zeros there
+    // the block that K ends in: the DMA takes its whole chunks (lanes beyond them fetch the start of their row instead: K is
+    // 16 or more), and behind the transfers' end those lanes write what belongs there, the rest of the row and zeros
+    const int64_t tail_left = k_len % kScaleBlock - schunk * 16;
+    auto stage_tail = [&](int64_t s, int buf) {
+        if constexpr (DMA) {
+            const unsigned base = lds0 + buf * STAGE;
+            const uint32_t k = tail_left >= 16 ? (uint32_t)(s * kScaleBlock) : 0u - schunk * 16;
+#pragma unroll
+            for (int i = 0; i < NA; ++i) lds_dma::dma16_split(A, a_off[i] + k, base + i * (T * 16));
+#pragma unroll
+            for (int i = 0; i < NB; ++i) lds_dma::dma16_split(B, b_off[i] + k, base + BM * 128 + i * (T * 16));
+        } else {
+            stage(s, buf);
+        }
+    };
     auto mend_tail = [&](int64_t s, int buf) {
         if constexpr (DMA) {
-            const int64_t k = it.k_begin + s * kScaleBlock + schunk * 16;
-            const int64_t left = it.k_end - k;
-            if (left > 0 && left < 16) {
+            if (tail_left >= 16) return;
+            uint8_t *to = image + buf * STAGE + srow * 128 + slot * 16;
+            const int64_t k = s * kScaleBlock + schunk * 16;
 #pragma unroll 1
-                for (int i = 0; i < NA; ++i)
-                    *reinterpret_cast<uint4 *>(&image[buf][(srow + i * (T / 8)) * 128 + slot * 16]) = load_chunk(A + a_off[i], k, it.k_end);
-#pragma unroll 1
-                for (int i = 0; i < NB; ++i)
-                    *reinterpret_cast<uint4 *>(&image[buf][BM * 128 + (srow + i * (T / 8)) * 128 + slot * 16]) = load_chunk(B + b_off[i], k, it.k_end);
+            for (int i = 0; i < NA + NB; ++i) {
+                const uint8_t *row = i < NA ? A + (int64_t)min(srow + i * (T / 8), a_last) * p.a.ld : B + (int64_t)min(srow + (i - NA) * (T / 8), b_last) * p.b.ld;
+                *reinterpret_cast<uint4 *>(to + (i < NA ? i * (T * 16) : BM * 128 + (i - NA) * (T * 16))) = load_chunk(row, k, k_len);
             }
         }
     };
-    // scales: thread t owns entry t (+ T) of the tile's BM rows and BN columns
-    constexpr int NS = (BM + BN + T - 1) / T;
-    const float *s_ptr[NS];
-    int64_t s_blk[NS];
-    float s_val[NS];
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        const int e = t + i * T;
-        if (e < BM) {
-            int64_t r = it.m0 + e;
-            r = r < it.m_end ? r : it.m_end - 1;
-            s_ptr[i] = SA + (r >> p.a.shift) * p.a.s_row + blk0 * p.a.s_blk;
-            s_blk[i] = p.a.s_blk;
-        } else {
-            int64_t r = it.n0 + e - BM;
-            r = r < p.N ? r : p.N - 1;
-            s_ptr[i] = SB + (r >> p.b.shift) * p.b.s_row + blk0 * p.b.s_blk;
-            s_blk[i] = p.b.s_blk;
-        }
+    const int64_t whole = k_len / kScaleBlock;  // blocks in front of the one K ends in, if it ends in one
+    // scales: thread t owns entry t of the tile's BM rows and BN columns
+    const bool a_scale = wave < BM / 64;
+    const float *s_ptr;
+    int64_t s_step;
+    if (a_scale) {
+        s_ptr = p.a.scale + a_entry * p.a.s_batch + ((it.m0 + min(t, a_last)) >> p.a.shift) * p.a.s_row + blk0 * p.a.s_blk;
+        s_step = p.a.s_blk;
+    } else {
+        s_ptr = p.b.scale + b_entry * p.b.s_batch + ((it.n0 + min(t - BM, b_last)) >> p.b.shift) * p.b.s_row + blk0 * p.b.s_blk;
+        s_step = p.b.s_blk;
     }
-    auto scale_load = [&](int64_t s) {
-#pragma unroll
-        for (int i = 0; i < NS; ++i) s_val[i] = s_ptr[i][s * s_blk[i]];
-    };
-    auto scale_store = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-            if (NS * T == BM + BN || t + i * T < BM + BN) scales[buf][t + i * T] = s_val[i];
-    };
 
     v4f acc[MT][NT];
 #pragma unroll
@@ -253,31 +270,39 @@ __global__ void __launch_bounds__(WM *WN * 64) scaled_gemm_kernel(ScaledGemmPara
         for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 
     if (steps > 0) {
-        scale_load(0);
-        stage(0, 0);
-        scale_store(0);
+        const float v = *s_ptr;
+        s_ptr += s_step;
+        if (whole > 0) stage(0, 0);
+        else stage_tail(0, 0);
+        scales[t] = v;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (steps == 1) mend_tail(0, 0);
+        if (whole == 0) mend_tail(0, 0);
         __syncthreads();
     }
     const int fr = lane & 15, fg = lane >> 4;
     // fragment addresses: row base + fr, chunks fg and fg + 4 under the row's swizzle (fr / 2 & 7: row bases are multiples of 16)
     const int sw = (fr >> 1) & 7;
     const int off0 = fr * 128 + ((fg ^ sw) << 4), off1 = fr * 128 + (((fg + 4) ^ sw) << 4);
-    auto frag = [&](auto &f, const uint8_t *base) { f.set(*reinterpret_cast<const v4i *>(base + off0), *reinterpret_cast<const v4i *>(base + off1)); };
 #pragma unroll 1
     for (int64_t s = 0; s < steps; ++s) {
         const int buf = (int)(s & 1);
         const bool more = s + 1 < steps;
+        float s_next = 0.f;
         if (more) {
-            scale_load(s + 1);
-            stage(s + 1, buf ^ 1);
+            s_next = *s_ptr;
+            s_ptr += s_step;
+            if (s + 1 < whole) stage(s + 1, buf ^ 1);
+            else stage_tail(s + 1, buf ^ 1);
         }
-        const uint8_t *ia = &image[buf][wm * WTM * 128], *ib = &image[buf][BM * 128 + wn * WTN * 128];
-        const float *fs = scales[buf];
+        const uint8_t *stage_base = image + buf * STAGE;
+        const uint8_t *ia0 = stage_base + wm * WTM * 128 + off0, *ia1 = stage_base + wm * WTM * 128 + off1;
+        const uint8_t *ib0 = stage_base + (BM + wn * WTN) * 128 + off0, *ib1 = stage_base + (BM + wn * WTN) * 128 + off1;
+        const float *fs = scales + buf * (BM + BN);
         BlockOperand<0, FAST> fb[NT];
+        BlockOperand<FA, FAST> fa[2];
+        fa[0].set(*reinterpret_cast<const v4i *>(ia0), *reinterpret_cast<const v4i *>(ia1));
 #pragma unroll
-        for (int j = 0; j < NT; ++j) frag(fb[j], ib + j * 16 * 128);
+        for (int j = 0; j < NT; ++j) fb[j].set(*reinterpret_cast<const v4i *>(ib0 + j * 2048), *reinterpret_cast<const v4i *>(ib1 + j * 2048));
         v4f sb[BUNI ? 1 : NT];
         if constexpr (BUNI) {
             sb[0][0] = fs[BM + wn * WTN];
@@ -285,63 +310,68 @@ __global__ void __launch_bounds__(WM *WN * 64) scaled_gemm_kernel(ScaledGemmPara
 #pragma unroll
             for (int j = 0; j < NT; ++j) sb[j] = *reinterpret_cast<const v4f *>(fs + BM + wn * WTN + j * 16 + fg * 4);
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            BlockOperand<FA, FAST> fa;
-            frag(fa, ia + i * 16 * 128);
-            float sa = fs[wm * WTM + i * 16 + fr];
-            if constexpr (BUNI) sa *= sb[0][0];
-            v4f d[NT];
+        float sa[MT];
+        sa[0] = fs[wm * WTM + fr];
+        v4f d[2][NT];
+        auto add = [&](int i, const v4f(&v)[NT], float f) {
+            if constexpr (BUNI) f *= sb[0][0];
 #pragma unroll
             for (int j = 0; j < NT; ++j)
-                d[j] = block_sums<FA, FAST>(fb[j], fa);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
+                for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[j][r], BUNI ? f : f * sb[BUNI ? 0 : j][r], acc[i][j][r]);
+            // here and not where the sums are next used: the compiler would move the additions behind the whole block's MFMAs,
+            // with every tile's results live until then
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float f = BUNI ? sa : sa * sb[BUNI ? 0 : j][r];
-                    acc[i][j][r] = __builtin_fmaf(d[j][r], f, acc[i][j][r]);
-                }
+            for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[i][j]));
+        };
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            if (i + 1 < MT) {
+                fa[(i + 1) & 1].set(*reinterpret_cast<const v4i *>(ia0 + (i + 1) * 2048), *reinterpret_cast<const v4i *>(ia1 + (i + 1) * 2048));
+                sa[i + 1] = fs[wm * WTM + (i + 1) * 16 + fr];
             }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) d[i & 1][j] = block_sums<FA, FAST>(fb[j], fa[i & 1]);
+            if (i > 0) add(i - 1, d[(i - 1) & 1], sa[i - 1]);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        add(MT - 1, d[(MT - 1) & 1], sa[MT - 1]);
         if (more) {
-            scale_store(buf ^ 1);
+            scales[(buf ^ 1) * (BM + BN) + t] = s_next;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (s + 2 == steps) mend_tail(s + 1, buf ^ 1);
+            if (s + 1 == whole) mend_tail(s + 1, buf ^ 1);
         }
         __syncthreads();
     }
 
-    const int64_t n_base = it.n0 + wn * WTN + fg * 4;
-    if (p.split > 1) {
-        float *w = p.ws + ((int64_t)it.chunk * p.batch + it.entry) * p.M * p.N;
+    // The finished tile passes through LDS (the operands' stages are free) in pieces of 32 rows of every wave row, and
+    // leaves in runs of whole rows: 16 bytes or more per lane, a row's columns along the lanes.
+    constexpr int PITCH = BN + 4;  // the sixteen rows of a wave's store start on sixteen different 16-byte slots
+    static_assert(WM * 32 * PITCH * 4 <= 2 * STAGE && MT % 2 == 0, "a piece fits the stages");
+    float *piece = reinterpret_cast<float *>(image);
+    const int64_t c_entry = p.split > 1 ? 0 : p.mode == kScaledRows ? 0 : it.entry * p.c_batch;
+    float *ws = p.ws + ((int64_t)it.chunk * p.batch + it.entry) * p.M * p.N;
+    const bool vec = p.split > 1 ? (p.N & 3) == 0
+                                 : ((p.ldc | p.c_batch) & 3) == 0 && (reinterpret_cast<uintptr_t>(p.C) & (p.c_f32 ? 15 : 7)) == 0;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const int64_t m = it.m0 + wm * WTM + i * 16 + fr;
-            if (m >= it.m_end) continue;
+    for (int h = 0; h < MT / 2; ++h) {
+        if (h > 0) __syncthreads();
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int64_t n = n_base + j * 16;
-                float *c = w + m * p.N + n;
-                if ((p.N & 3) == 0 && n < p.N) *reinterpret_cast<v4f *>(c) = acc[i][j];
-                else
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (n + r < p.N) c[r] = acc[i][j][r];
-            }
-        }
-        return;
-    }
-    const int64_t c_entry = p.mode == kScaledRows ? 0 : it.entry * p.c_batch;
-    const bool vec = ((p.ldc | p.c_batch) & 3) == 0 && (reinterpret_cast<uintptr_t>(p.C) & (p.c_f32 ? 15 : 7)) == 0;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int64_t m = it.m0 + wm * WTM + i * 16 + fr;
-        if (m >= it.m_end) continue;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int64_t n = n_base + j * 16;
-            if (n < p.N) store4(p, c_entry + m * p.ldc + n, n, acc[i][j], vec);
+            for (int j = 0; j < NT; ++j)
+                *reinterpret_cast<v4f *>(piece + (wm * 32 + i * 16 + fr) * PITCH + wn * WTN + j * 16 + fg * 4) = acc[2 * h + i][j];
+        __syncthreads();
+        constexpr int QUADS = BN / 4, STEP = T / QUADS;
+        const int q = t % QUADS;
+        const int64_t n = it.n0 + q * 4;
+#pragma unroll 2
+        for (int r = t / QUADS; r < WM * 32; r += STEP) {
+            const int64_t m = it.m0 + (r >> 5) * WTM + h * 32 + (r & 31);
+            if (m >= it.m_end || n >= p.N) continue;
+            const v4f v = *reinterpret_cast<const v4f *>(piece + r * PITCH + q * 4);
+            if (p.split > 1) store_partial(ws + m * p.N + n, p.N - n, v, vec);
+            else store4(p, c_entry + m * p.ldc + n, n, v, vec);
         }
     }
 }
@@ -380,7 +410,8 @@ template <int FA, bool FAST, bool BUNI> hipError_t launch_tiles(const ScaledGemm
     return hipGetLastError();
 }
 
-bool dma_ready(const ScaledMatrix &m) { return ((reinterpret_cast<uintptr_t>(m.q) | (uintptr_t)m.ld | (uintptr_t)m.batch) & 15) == 0; }
+// (2^22: the DMA's offsets inside a tile are 32-bit, 255 rows and a row's length)
+bool dma_ready(const ScaledMatrix &m, int64_t k) { return ((reinterpret_cast<uintptr_t>(m.q) | (uintptr_t)m.ld | (uintptr_t)m.batch) & 15) == 0 && m.ld <= 1 << 22 && k >= 16; }
 
 }  // namespace
 
@@ -394,7 +425,7 @@ ScaledSchedule schedule_scaled(const ScaledGemmParams &p, int cus, size_t ws_lim
         const int64_t nbm = (p.M + b - 1) / b + (p.mode == kScaledRows ? p.batch / 2 : 0);
         return nbm * ((p.N + b - 1) / b) * entries;
     };
-    s.kind = !p.c_f32 && dma_ready(p.a) && dma_ready(p.b) && tiles(256) >= cus * 3 / 4 ? 2 : 1;
+    s.kind = !p.c_f32 && dma_ready(p.a, p.K) && dma_ready(p.b, p.K) && tiles(256) >= cus * 3 / 4 ? 2 : 1;
     if (s.kind == 1 && p.mode == kScaledDense && tiles(128) < cus) {
         const int64_t steps = (p.K + kScaleBlock - 1) / kScaleBlock;
         int64_t split = 2 * cus / tiles(128);
@@ -422,7 +453,7 @@ hipError_t launch_scaled_gemm(ScaledGemmParams p, const ScaledSchedule &s, hipSt
     // row tiles of ragged groups: each group adds at most one partly filled tile
     if (p.mode == kScaledRows) grid = (p.M / b + (p.batch < p.M ? p.batch : p.M)) * (int64_t)p.nbn;
     if (grid > 0x7fffff) return hipErrorInvalidValue;
-    const bool uni = p.b.shift == 7, dma = dma_ready(p.a) && dma_ready(p.b);
+    const bool uni = p.b.shift == 7, dma = dma_ready(p.a, p.K) && dma_ready(p.b, p.K);
     const bool fast = !p.c_f32;  // an f32 result takes f32 sums (see block_sums)
     typedef hipError_t (*launcher)(const ScaledGemmParams &, int, bool, unsigned, hipStream_t);
     static const launcher table[2][2][2] = {{{launch_tiles<0, false, false>, launch_tiles<0, false, true>}, {launch_tiles<0, true, false>, launch_tiles<0, true, true>}},
