@@ -24,13 +24,21 @@ int unsupported(const char *what, const char *why) { return set_last_error(CTC_T
 
 int64_t blocks_of(int64_t n) { return (n + ctc::kScaleBlock - 1) / ctc::kScaleBlock; }
 
+// of the current device; asked for once per device
 int compute_units()
 {
+    static std::atomic<int> known[64];
     int dev = 0, cus = 0;
-    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1) {
+    if (hipGetDevice(&dev) != hipSuccess) {
         (void)hipGetLastError();
         return 256;
     }
+    if (dev >= 0 && dev < 64 && (cus = known[dev].load(std::memory_order_relaxed)) > 0) return cus;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus < 1) {
+        (void)hipGetLastError();
+        return 256;
+    }
+    if (dev >= 0 && dev < 64) known[dev].store(cus, std::memory_order_relaxed);
     return cus;
 }
 
