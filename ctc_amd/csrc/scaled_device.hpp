@@ -48,17 +48,20 @@ template <int FMT> struct BlockOperand<FMT, false> {
         v[3] = widen<FMT>(hi[2], hi[3]);
     }
 };
-// the 16 x 16 sums of a block's products (rows of B x rows of A)
-template <int FA, bool FAST> __device__ __forceinline__ v4f block_sums(const BlockOperand<0, FAST> &b, const BlockOperand<FA, FAST> &a)
+// the 16 x 16 sums of a block's products: NT row tiles of B by one of A
+template <int FA, bool FAST, int NT> __device__ __forceinline__ void block_sums(const BlockOperand<0, FAST> (&b)[NT], const BlockOperand<FA, FAST> &a, v4f (&d)[NT])
 {
-    v4f d = {0.f, 0.f, 0.f, 0.f};
+    const v4f zero = {0.f, 0.f, 0.f, 0.f};
     if constexpr (FAST) {
-        d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b.v, a.v, d, 0, FA, 0, 0, 0, 0);
-    } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.v[q], a.v[q], d, 0, 0, 0);
+        for (int j = 0; j < NT; ++j) d[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j].v, a.v, zero, 0, FA, 0, 0, 0, 0);
+    } else {
+        // a quarter of every tile before the next quarter: the MFMAs of one tile depend on each other
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) d[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j].v[q], a.v[q], q ? d[j] : zero, 0, 0, 0);
     }
-    return d;
 }
 
 // 16 bytes of a row from byte k on, zeros from byte k_end on; any alignment

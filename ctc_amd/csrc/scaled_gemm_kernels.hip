@@ -279,6 +279,8 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmP
         if (whole == 0) mend_tail(0, 0);
         __syncthreads();
     }
+    // a wave whose rows all lie behind the last one only stages: a group's last tile with at most half of its rows takes half the time
+    const bool active = it.m0 + wm * WTM < it.m_end;
     const int fr = lane & 15, fg = lane >> 4;
     // fragment addresses: row base + fr, chunks fg and fg + 4 under the row's swizzle (fr / 2 & 7: row bases are multiples of 16)
     const int sw = (fr >> 1) & 7;
@@ -294,48 +296,57 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmP
             if (s + 1 < whole) stage(s + 1, buf ^ 1);
             else stage_tail(s + 1, buf ^ 1);
         }
-        const uint8_t *stage_base = image + buf * STAGE;
-        const uint8_t *ia0 = stage_base + wm * WTM * 128 + off0, *ia1 = stage_base + wm * WTM * 128 + off1;
-        const uint8_t *ib0 = stage_base + (BM + wn * WTN) * 128 + off0, *ib1 = stage_base + (BM + wn * WTN) * 128 + off1;
-        const float *fs = scales + buf * (BM + BN);
-        BlockOperand<0, FAST> fb[NT];
-        BlockOperand<FA, FAST> fa[2];
-        fa[0].set(*reinterpret_cast<const v4i *>(ia0), *reinterpret_cast<const v4i *>(ia1));
+        if (active) {
+            const uint8_t *stage_base = image + buf * STAGE;
+            const uint8_t *ia0 = stage_base + wm * WTM * 128 + off0, *ia1 = stage_base + wm * WTM * 128 + off1;
+            const uint8_t *ib0 = stage_base + (BM + wn * WTN) * 128 + off0, *ib1 = stage_base + (BM + wn * WTN) * 128 + off1;
+            const float *fs = scales + buf * (BM + BN);
+            BlockOperand<0, FAST> fb[NT];
+            BlockOperand<FA, FAST> fa[2];
+            fa[0].set(*reinterpret_cast<const v4i *>(ia0), *reinterpret_cast<const v4i *>(ia1));
 #pragma unroll
-        for (int j = 0; j < NT; ++j) fb[j].set(*reinterpret_cast<const v4i *>(ib0 + j * 2048), *reinterpret_cast<const v4i *>(ib1 + j * 2048));
-        v4f sb[BUNI ? 1 : NT];
-        if constexpr (BUNI) {
-            sb[0][0] = fs[BM + wn * WTN];
-        } else {
+            for (int j = 0; j < NT; ++j) fb[j].set(*reinterpret_cast<const v4i *>(ib0 + j * 2048), *reinterpret_cast<const v4i *>(ib1 + j * 2048));
+            v4f sb[BUNI ? 1 : NT];
+            if constexpr (BUNI) {
+                sb[0][0] = fs[BM + wn * WTN];
+            } else {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) sb[j] = *reinterpret_cast<const v4f *>(fs + BM + wn * WTN + j * 16 + fg * 4);
-        }
-        float sa[MT];
-        sa[0] = fs[wm * WTM + fr];
-        v4f d[2][NT];
-        auto add = [&](int i, const v4f(&v)[NT], float f) {
-            if constexpr (BUNI) f *= sb[0][0];
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[j][r], BUNI ? f : f * sb[BUNI ? 0 : j][r], acc[i][j][r]);
-            // here and not where the sums are next used: the compiler would move the additions behind the whole block's MFMAs,
-            // with every tile's results live until then
-#pragma unroll
-            for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[i][j]));
-        };
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            if (i + 1 < MT) {
-                fa[(i + 1) & 1].set(*reinterpret_cast<const v4i *>(ia0 + (i + 1) * 2048), *reinterpret_cast<const v4i *>(ia1 + (i + 1) * 2048));
-                sa[i + 1] = fs[wm * WTM + (i + 1) * 16 + fr];
+                for (int j = 0; j < NT; ++j) sb[j] = *reinterpret_cast<const v4f *>(fs + BM + wn * WTN + j * 16 + fg * 4);
             }
+            float sa[MT];
+            sa[0] = fs[wm * WTM + fr];
+            v4f d[2][NT];
+            auto add = [&](int i, const v4f(&v)[NT], float f) {
+                if constexpr (BUNI) f *= sb[0][0];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) d[i & 1][j] = block_sums<FA, FAST>(fb[j], fa[i & 1]);
-            if (i > 0) add(i - 1, d[(i - 1) & 1], sa[i - 1]);
-            __builtin_amdgcn_sched_barrier(0);
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[j][r], BUNI ? f : f * sb[BUNI ? 0 : j][r], acc[i][j][r]);
+                // here and not where the sums are next used: the compiler would move the additions behind the whole block's MFMAs,
+                // with every tile's results live until then
+#pragma unroll
+                for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[i][j]));
+            };
+            if constexpr (!FAST) __builtin_amdgcn_s_setprio(1);  // (4 % here, nothing for the 8-bit form)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                if (i + 1 < MT) {
+                    fa[(i + 1) & 1].set(*reinterpret_cast<const v4i *>(ia0 + (i + 1) * 2048), *reinterpret_cast<const v4i *>(ia1 + (i + 1) * 2048));
+                    sa[i + 1] = fs[wm * WTM + (i + 1) * 16 + fr];
+                }
+                block_sums<FA, FAST, NT>(fb, fa[i & 1], d[i & 1]);
+                if (i > 0) add(i - 1, d[(i - 1) & 1], sa[i - 1]);
+                // one MFMA, then additions: a wave that waits for the matrix core has work, and the core always a request
+#pragma unroll
+                for (int j = 0; j < (FAST ? NT : 4 * NT); ++j) {
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x2, FAST ? (BUNI ? 5 : 8) : (BUNI ? 2 : 3), 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (!FAST) __builtin_amdgcn_s_setprio(0);
+            add(MT - 1, d[(MT - 1) & 1], sa[MT - 1]);
         }
-        add(MT - 1, d[(MT - 1) & 1], sa[MT - 1]);
         if (more) {
             scales[(buf ^ 1) * (BM + BN) + t] = s_next;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

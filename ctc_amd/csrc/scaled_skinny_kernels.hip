@@ -97,16 +97,17 @@ template <int FA, bool BUNI, int MT, int NW> __global__ void __launch_bounds__(N
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (s0 + u * NW >= steps) break;
-                BlockOperand<0, false> ob;
-                ob.set(fb[u].lo, fb[u].hi);
+                BlockOperand<0, false> ob[1];
+                ob[0].set(fb[u].lo, fb[u].hi);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
                     if (i > 0 && rows <= i * 16) break;
                     BlockOperand<FA, false> oa;
                     oa.set(fa[u][i].lo, fa[u][i].hi);
-                    const v4f d = block_sums<FA, false>(ob, oa);
+                    v4f d[1];
+                    block_sums<FA, false, 1>(ob, oa, d);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[i][r] = __builtin_fmaf(d[r], sa[u][i] * sb[u][BUNI ? 0 : r], acc[i][r]);
+                    for (int r = 0; r < 4; ++r) acc[i][r] = __builtin_fmaf(d[0][r], sa[u][i] * sb[u][BUNI ? 0 : r], acc[i][r]);
                 }
             }
         }
