@@ -20,13 +20,6 @@ constexpr float kFloor = 7.8886090522101181e-31f;  // 2^-100
 
 template <int FMT> constexpr float largest() { return FMT ? 57344.f : 448.f; }
 
-// |x| of a finite x, 0 otherwise
-__device__ __forceinline__ float finite_mag(float x)
-{
-    const float a = __builtin_fabsf(x);
-    return a < __builtin_inff() ? a : 0.f;  // false for NaN
-}
-
 template <int FMT> __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d)
 {
     int v = 0;
@@ -40,33 +33,59 @@ template <int FMT> __device__ __forceinline__ uint32_t pack4(float a, float b, f
     return (uint32_t)v;
 }
 
-// eight consecutive elements of a row from column c on, zeros beyond `cols`
-template <int SRC> __device__ __forceinline__ void load8(const void *x, int64_t at, int64_t c, int64_t cols, float (&v)[8])
-{
-    if (c + 8 <= cols) {
-        if constexpr (SRC == 2) {
-            uint4 u;
-            __builtin_memcpy(&u, static_cast<const uint16_t *>(x) + at, 16);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16);
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-        } else {
-            __builtin_memcpy(v, static_cast<const float *>(x) + at, 32);
-        }
-        return;
+// Eight consecutive elements of a row as they lie in memory.  Magnitudes are compared as integers, two bf16 at a time:
+// without their signs, finite numbers order like their bits and infinities and NaNs stand above them.
+template <int SRC> struct Row8;
+template <> struct Row8<2> {
+    static constexpr int W = 4;
+    static constexpr uint32_t kSigns = 0x80008000u;
+    uint32_t w[4];
+    static __device__ __forceinline__ uint32_t pmax(uint32_t a, uint32_t b)
+    {
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        v[i] = 0.f;
-        if (c + i < cols) {
-            if constexpr (SRC == 2) v[i] = __uint_as_float((uint32_t)static_cast<const uint16_t *>(x)[at + i] << 16);
-            else v[i] = static_cast<const float *>(x)[at + i];
-        }
+    static __device__ __forceinline__ uint32_t fold(uint32_t m) { return max(m & 0xffffu, m >> 16); }  // of both halves
+    static __device__ __forceinline__ uint32_t finite(uint32_t m)
+    {
+        return ((m & 0xffffu) < 0x7f80u ? m & 0xffffu : 0u) | (m < 0x7f800000u ? m & 0xffff0000u : 0u);
     }
-}
+    static __device__ __forceinline__ bool special(uint32_t m) { return fold(m) >= 0x7f80u; }
+    static __device__ __forceinline__ float value(uint32_t m) { return __uint_as_float(m << 16); }  // of a folded maximum
+    __device__ __forceinline__ float at(int j) const { return __uint_as_float(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16); }
+    __device__ __forceinline__ void load(const void *x, int64_t at, int64_t left)
+    {
+        const uint16_t *p = static_cast<const uint16_t *>(x) + at;
+        if (left >= 8) {
+            __builtin_memcpy(w, p, 16);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[i] = (2 * i < left ? (uint32_t)p[2 * i] : 0u) | (2 * i + 1 < left ? (uint32_t)p[2 * i + 1] << 16 : 0u);
+    }
+};
+template <> struct Row8<1> {
+    static constexpr int W = 8;
+    static constexpr uint32_t kSigns = 0x80000000u;
+    uint32_t w[8];
+    static __device__ __forceinline__ uint32_t pmax(uint32_t a, uint32_t b) { return max(a, b); }
+    static __device__ __forceinline__ uint32_t fold(uint32_t m) { return m; }
+    static __device__ __forceinline__ uint32_t finite(uint32_t m) { return m < 0x7f800000u ? m : 0u; }
+    static __device__ __forceinline__ bool special(uint32_t m) { return m >= 0x7f800000u; }
+    static __device__ __forceinline__ float value(uint32_t m) { return __uint_as_float(m); }
+    __device__ __forceinline__ float at(int j) const { return __uint_as_float(w[j]); }
+    __device__ __forceinline__ void load(const void *x, int64_t at, int64_t left)
+    {
+        const uint32_t *p = static_cast<const uint32_t *>(x) + at;
+        if (left >= 8) {
+            __builtin_memcpy(w, p, 32);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = i < left ? p[i] : 0u;
+    }
+};
 
 // eight codes to q[0 .. 8), those with an index below n only
 __device__ __forceinline__ void store8(uint8_t *q, uint32_t lo, uint32_t hi, int64_t n)
@@ -81,17 +100,20 @@ __device__ __forceinline__ void store8(uint8_t *q, uint32_t lo, uint32_t hi, int
         if (i < n) q[i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
 }
 
-__device__ __forceinline__ float max16(float m)
+// the maximum over the sixteen lanes of a DPP row, in all of them
+template <typename R> __device__ __forceinline__ uint32_t max16(uint32_t m)
 {
-#pragma unroll
-    for (int d = 1; d < 16; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-    return m;
+    m = R::pmax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x128, 0xf, 0xf, false));  // row_ror 8, 4, 2, 1
+    m = R::pmax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x124, 0xf, 0xf, false));
+    m = R::pmax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x122, 0xf, 0xf, false));
+    return R::pmax(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x121, 0xf, 0xf, false));
 }
 
 // One scale per row and 128 columns, no transpose: sixteen lanes own a group and load it whole (16 or 32 bytes a lane),
 // so the maximum is four exchanges inside sixteen lanes and nothing passes through LDS.
 template <int SRC, int FMT> __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantizeParams p, int64_t nblk, int64_t total)
 {
+    typedef Row8<SRC> R;
     const int64_t first = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
     const int64_t step = (int64_t)gridDim.x * 16;
     const int lane = threadIdx.x & 15;
@@ -99,110 +121,114 @@ template <int SRC, int FMT> __global__ void __launch_bounds__(256) quantize_rows
         const int64_t blk = g % nblk, rest = g / nblk;
         const int64_t row = rest % p.rows, b = rest / p.rows;
         const int64_t c = blk * kScaleBlock + lane * 8;
-        float v[8];
-        load8<SRC>(p.x, b * p.x_batch + row * p.ldx + c, c, p.cols, v);
-        float m = 0.f;
+        R v;
+        v.load(p.x, b * p.x_batch + row * p.ldx + c, p.cols - c);
+        uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_mag(v[i]));
-        const float top = fmaxf(max16(m), kFloor);
+        for (int i = 0; i < R::W; ++i) m = R::pmax(m, v.w[i] & ~R::kSigns);
+        if (__any(R::special(m))) {
+            m = 0;
+#pragma unroll
+            for (int i = 0; i < R::W; ++i) m = R::pmax(m, R::finite(v.w[i] & ~R::kSigns));
+        }
+        const float top = fmaxf(R::value(R::fold(max16<R>(m))), kFloor);
         const float r = largest<FMT>() / top;
-        const uint32_t lo = pack4<FMT>(v[0] * r, v[1] * r, v[2] * r, v[3] * r);
-        const uint32_t hi = pack4<FMT>(v[4] * r, v[5] * r, v[6] * r, v[7] * r);
+        const uint32_t lo = pack4<FMT>(v.at(0) * r, v.at(1) * r, v.at(2) * r, v.at(3) * r);
+        const uint32_t hi = pack4<FMT>(v.at(4) * r, v.at(5) * r, v.at(6) * r, v.at(7) * r);
         store8(p.out.q + b * p.out.batch + row * p.out.ld + c, lo, hi, p.cols - c);
         if (lane == 0) p.out.scale[b * p.out.s_batch + row * p.out.s_row + blk * p.out.s_blk] = top / largest<FMT>();
     }
 }
 
-// A 128 x 128 tile per workgroup, held in registers: thread (rg, cg) owns an 8 x 8 block (rows 8 rg .., columns 8 cg ..),
-// so a row's maximum is an exchange inside sixteen lanes, a column's one between the four row groups of a wave and one
-// pass through LDS between the waves, and a block's eight column slices are the eight bytes that the transposed
-// row takes: one 8-byte LDS store each, no byte shuffles through memory.  The transposed tile leaves LDS in 16-byte rows.
-template <int SRC, int FMT, bool TILES> __global__ void __launch_bounds__(256) quantize_tile_kernel(QuantizeParams p, unsigned nblk)
+// A 128 x 128 tile per workgroup, held in registers as it was loaded: thread (rg, cg) owns an 8 x 8 block (rows 8 rg ..,
+// columns 8 cg ..), so a row's maximum is an exchange inside sixteen lanes, a column's one between the four row groups of
+// a wave and one pass through LDS between the waves, and a block's eight column slices are the eight bytes that the
+// transposed row takes: one 8-byte LDS store each, no byte shuffles through memory.  The transposed tile leaves LDS in
+// 16-byte rows.  bf16: at most 128 registers, four workgroups a CU,
+// whose loads, exchanges and stores cover each other (8192 x 4096, both ways: 29.4 us, 4.7 TB/s; with two workgroups 44);
+// f32 spills there and takes three (5001 x 4104 tiles, both ways: 31 us, 3.9 TB/s; with four and spills 45).
+template <int SRC, int FMT, bool TILES> __global__ void __launch_bounds__(256, SRC == 2 ? 4 : 3) quantize_tile_kernel(QuantizeParams p, unsigned nblk)
 {
+    typedef Row8<SRC> R;
     __shared__ __attribute__((aligned(16))) uint8_t image[128 * 128];
-    __shared__ float part[4][128];
-    __shared__ float part_tile[4];
+    __shared__ uint32_t part[4][16 * R::W];
+    __shared__ uint32_t part_tile[4];
     const int t = threadIdx.x, cg = t & 15, rg = t >> 4, wave = t >> 6;
     const int64_t cblk = blockIdx.x % nblk, rblk = blockIdx.x / nblk;
     const int64_t c0 = cblk * 128 + cg * 8, r0 = rblk * 128 + rg * 8;
     const int64_t b = blockIdx.z;
     const bool rowwise = p.out.q != nullptr, transposed = p.out_t.q != nullptr;
 
-    float v[8][8];  // [row][column]
+    R v[8];
+    const int64_t x0 = b * p.x_batch + r0 * p.ldx + c0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int64_t row = r0 + i;
-        if (row < p.rows && c0 < p.cols) {
-            load8<SRC>(p.x, b * p.x_batch + row * p.ldx + c0, c0, p.cols, v[i]);
-        } else {
+    for (int i = 0; i < 8; ++i) v[i].load(p.x, x0 + i * p.ldx, r0 + i < p.rows ? p.cols - c0 : 0);
+    uint32_t rmax[8], cmax[R::W];
+    auto maxima = [&](auto filter) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        for (int j = 0; j < R::W; ++j) cmax[j] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            rmax[i] = 0;
+#pragma unroll
+            for (int j = 0; j < R::W; ++j) {
+                const uint32_t m = filter(v[i].w[j] & ~R::kSigns);
+                rmax[i] = R::pmax(rmax[i], m);
+                cmax[j] = R::pmax(cmax[j], m);
+            }
         }
-    }
-    float rmax[8], cmax[8];
+    };
+    maxima([](uint32_t m) { return m; });
+    uint32_t all = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) cmax[j] = 0.f;
+    for (int j = 0; j < R::W; ++j) all = R::pmax(all, cmax[j]);
+    if (__any(R::special(all))) {
+        maxima([](uint32_t m) { return R::finite(m); });
+        all = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        rmax[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float m = finite_mag(v[i][j]);
-            rmax[i] = fmaxf(rmax[i], m);
-            cmax[j] = fmaxf(cmax[j], m);
-        }
+        for (int j = 0; j < R::W; ++j) all = R::pmax(all, cmax[j]);
     }
     float tile_top = kFloor;
     if constexpr (TILES) {
-        float m = rmax[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) m = fmaxf(m, rmax[i]);
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+        uint32_t m = R::fold(max16<R>(all));
+        m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+        m = max(m, (uint32_t)__shfl_xor((int)m, 32));
         if ((t & 63) == 0) part_tile[wave] = m;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 4; ++w) tile_top = fmaxf(tile_top, part_tile[w]);
+        for (int w = 0; w < 4; ++w) tile_top = fmaxf(tile_top, R::value(part_tile[w]));
     }
     if (rowwise) {
         float top = tile_top;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if constexpr (!TILES) top = fmaxf(max16(rmax[i]), kFloor);
+            if constexpr (!TILES) top = fmaxf(R::value(R::fold(max16<R>(rmax[i]))), kFloor);
             const float r = largest<FMT>() / top;
             const int64_t row = r0 + i;
             if (row < p.rows && c0 < p.cols) {
-                const uint32_t lo = pack4<FMT>(v[i][0] * r, v[i][1] * r, v[i][2] * r, v[i][3] * r);
-                const uint32_t hi = pack4<FMT>(v[i][4] * r, v[i][5] * r, v[i][6] * r, v[i][7] * r);
+                const uint32_t lo = pack4<FMT>(v[i].at(0) * r, v[i].at(1) * r, v[i].at(2) * r, v[i].at(3) * r);
+                const uint32_t hi = pack4<FMT>(v[i].at(4) * r, v[i].at(5) * r, v[i].at(6) * r, v[i].at(7) * r);
                 store8(p.out.q + b * p.out.batch + row * p.out.ld + c0, lo, hi, p.cols - c0);
             }
-            if (!TILES && cg == 0 && row < p.rows)
-                p.out.scale[b * p.out.s_batch + row * p.out.s_row + cblk * p.out.s_blk] = top / largest<FMT>();
+            if (!TILES && cg == 0 && row < p.rows) p.out.scale[b * p.out.s_batch + row * p.out.s_row + cblk * p.out.s_blk] = top / largest<FMT>();
         }
-        if (TILES && t == 0)
-            p.out.scale[b * p.out.s_batch + rblk * p.out.s_row + cblk * p.out.s_blk] = tile_top / largest<FMT>();
+        if (TILES && t == 0) p.out.scale[b * p.out.s_batch + rblk * p.out.s_row + cblk * p.out.s_blk] = tile_top / largest<FMT>();
     }
     if (!transposed) return;
     if constexpr (!TILES) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            cmax[j] = fmaxf(cmax[j], __shfl_xor(cmax[j], 16));
-            cmax[j] = fmaxf(cmax[j], __shfl_xor(cmax[j], 32));
+        for (int j = 0; j < R::W; ++j) {
+            cmax[j] = R::pmax(cmax[j], (uint32_t)__shfl_xor((int)cmax[j], 16));
+            cmax[j] = R::pmax(cmax[j], (uint32_t)__shfl_xor((int)cmax[j], 32));
         }
         if ((t & 48) == 0) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) part[wave][cg * 8 + j] = cmax[j];
+            for (int j = 0; j < R::W; ++j) part[wave][cg * R::W + j] = cmax[j];
         }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            cmax[j] = fmaxf(fmaxf(fmaxf(part[0][cg * 8 + j], part[1][cg * 8 + j]), fmaxf(part[2][cg * 8 + j], part[3][cg * 8 + j])), kFloor);
-        if (rg == 0) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c0 + j < p.cols)
-                    p.out_t.scale[b * p.out_t.s_batch + (c0 + j) * p.out_t.s_row + rblk * p.out_t.s_blk] = cmax[j] / largest<FMT>();
-        }
+        for (int j = 0; j < R::W; ++j)
+            cmax[j] = R::pmax(R::pmax(part[0][cg * R::W + j], part[1][cg * R::W + j]), R::pmax(part[2][cg * R::W + j], part[3][cg * R::W + j]));
     } else if (t == 0) {
         p.out_t.scale[b * p.out_t.s_batch + cblk * p.out_t.s_row + rblk * p.out_t.s_blk] = tile_top / largest<FMT>();
     }
@@ -210,9 +236,14 @@ template <int SRC, int FMT, bool TILES> __global__ void __launch_bounds__(256) q
     // column 8 cg + j, lines a kilobyte apart, and would all meet in the same banks without it
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float r = largest<FMT>() / (TILES ? tile_top : cmax[j]);
-        const uint32_t lo = pack4<FMT>(v[0][j] * r, v[1][j] * r, v[2][j] * r, v[3][j] * r);
-        const uint32_t hi = pack4<FMT>(v[4][j] * r, v[5][j] * r, v[6][j] * r, v[7][j] * r);
+        float top = tile_top;
+        if constexpr (!TILES) {
+            top = fmaxf(R::value(SRC == 2 ? (j & 1 ? cmax[j >> 1] >> 16 : cmax[j >> 1] & 0xffffu) : cmax[j % R::W]), kFloor);
+            if (rg == 0 && c0 + j < p.cols) p.out_t.scale[b * p.out_t.s_batch + (c0 + j) * p.out_t.s_row + rblk * p.out_t.s_blk] = top / largest<FMT>();
+        }
+        const float r = largest<FMT>() / top;
+        const uint32_t lo = pack4<FMT>(v[0].at(j) * r, v[1].at(j) * r, v[2].at(j) * r, v[3].at(j) * r);
+        const uint32_t hi = pack4<FMT>(v[4].at(j) * r, v[5].at(j) * r, v[6].at(j) * r, v[7].at(j) * r);
         *reinterpret_cast<uint2 *>(image + (cg * 8 + j) * 128 + (((rg >> 1) ^ (cg & 7)) << 4) + ((rg & 1) << 3)) = make_uint2(lo, hi);
     }
     __syncthreads();
