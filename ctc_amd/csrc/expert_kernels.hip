@@ -17,45 +17,31 @@ using namespace scaled;
 
 namespace {
 
-constexpr int kWaves = 8;
 static_assert(kExpertMaxTokens == 64, "a token is a lane of a wave");
 static_assert(kExpertMaxExperts / 32 == 128, "a lane of the listing wave reads two words of the experts' bits");
 
-// one block of 128 contracted elements of a row, as a lane of group fg holds it: bytes k .. k + 16 and k + 64 .. k + 80
-struct Codes {
-    uint4 lo, hi;
-};
-__device__ __forceinline__ Codes load_codes(const uint8_t *row, int64_t k, int64_t k_end, bool whole)
-{
-    Codes c;
-    if (whole) {
-        __builtin_memcpy(&c.lo, row + k, 16);
-        __builtin_memcpy(&c.hi, row + k + 64, 16);
-    } else {
-        c.lo = load_chunk(row, k, k_end);
-        c.hi = load_chunk(row, k + 64, k_end);
-    }
-    return c;
-}
-// the bf16 elements at the same places
+// the bf16 elements at the places of a lane's Codes
 struct Halves {
     uint4 v[4];
 };
-__device__ __forceinline__ Halves load_halves(const uint8_t *row, int64_t k, int64_t k_end, bool whole)
+__device__ __forceinline__ Halves load_halves(const uint8_t *row, int64_t k)
 {
     Halves h;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int64_t at = 2 * (k + (q & 1) * 8 + (q >> 1) * 64);
-        if (whole) __builtin_memcpy(&h.v[q], row + at, 16);
-        else h.v[q] = load_chunk(row, at, 2 * k_end);
-    }
+    for (int q = 0; q < 4; ++q) __builtin_memcpy(&h.v[q], row + 2 * (k + (q & 1) * 8 + (q >> 1) * 64), 16);
+    return h;
+}
+__device__ __forceinline__ Halves load_last_halves(const uint8_t *row, int64_t k, int64_t k_end, bool long_row)
+{
+    Halves h;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) h.v[q] = load_chunk(row, 2 * (k + (q & 1) * 8 + (q >> 1) * 64), 2 * k_end, long_row);
     return h;
 }
 __device__ __forceinline__ v4f block_product(const Codes &c, const Halves &h)
 {
     v4f d = {0.f, 0.f, 0.f, 0.f};
-    const uint32_t w[8] = {c.lo.x, c.lo.y, c.lo.z, c.lo.w, c.hi.x, c.hi.y, c.hi.z, c.hi.w};
+    const uint32_t w[8] = {(uint32_t)c.lo[0], (uint32_t)c.lo[1], (uint32_t)c.lo[2], (uint32_t)c.lo[3], (uint32_t)c.hi[0], (uint32_t)c.hi[1], (uint32_t)c.hi[2], (uint32_t)c.hi[3]};
 #pragma unroll
     for (int q = 0; q < 4; ++q)
         d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen<0>(w[2 * q], w[2 * q + 1]), __builtin_bit_cast(bf16x8, h.v[q]), d, 0, 0, 0);
@@ -86,9 +72,10 @@ __device__ __forceinline__ int place_of(const Picks &k, int e)
 // h = gate * silu(G x) * (U x) for 16 of an expert's inner rows and all its tokens.  Workgroup (slice, y): y is a pair
 // (token, place) where there are fewer pairs than experts, and only the first pair of an expert works; else y is the expert.
 // Eight waves share the contracted blocks; their partial sums meet in LDS, in wave order.
-template <bool UNI> __global__ void __launch_bounds__(kWaves * 64) expert_up_kernel(ExpertParams p, int by_pair)
+template <bool UNI, int NW, int U> __global__ void __launch_bounds__(NW * 64) expert_up_kernel(ExpertParams p, int by_pair)
 {
-    __shared__ __attribute__((aligned(16))) float part[kWaves][2][256];
+    __shared__ __attribute__((aligned(16))) float part[NW][2][256];
+    __shared__ __attribute__((aligned(16))) uint8_t scratch[NW][2048];
     __shared__ int token_of[64], row_of[64];
     __shared__ float gate_of[64];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -119,63 +106,73 @@ template <bool UNI> __global__ void __launch_bounds__(kWaves * 64) expert_up_ker
     }
     __syncthreads();
 
-    const int64_t iu = i0 + fr < p.inner ? i0 + fr : p.inner - 1;
-    const uint8_t *w_gate = p.up.q + e * p.up.batch + iu * p.up.ld, *w_up = w_gate + p.inner * p.up.ld;
-    const float *S = p.up.scale + e * p.up.s_batch;
-    const float *s_gate[UNI ? 1 : 4], *s_up[UNI ? 1 : 4];
+    constexpr int S = UNI ? 1 : 4;
+    const uint8_t *W = p.up.q + e * p.up.batch;
+    const int64_t to_up = p.inner * p.up.ld;
+    const uint8_t *w_gate = W + min64(i0 + (lane >> 2), p.inner - 1) * p.up.ld + (lane & 3) * 16, *w_up = w_gate + to_up;
+    const float *scale = p.up.scale + e * p.up.s_batch;
+    const float *s_gate[S], *s_up[S];
 #pragma unroll
-    for (int r = 0; r < (UNI ? 1 : 4); ++r) {
+    for (int r = 0; r < S; ++r) {
         int64_t i = UNI ? i0 : i0 + fg * 4 + r;
         i = i < p.inner ? i : p.inner - 1;
-        s_gate[r] = S + (i >> 7) * p.up.s_row;
-        s_up[r] = S + ((p.inner + i) >> 7) * p.up.s_row;
+        s_gate[r] = scale + (i >> 7) * p.up.s_row;
+        s_up[r] = scale + ((p.inner + i) >> 7) * p.up.s_row;
     }
-    const int steps = (int)((p.hidden + kScaleBlock - 1) / kScaleBlock);
+    const int whole = (int)(p.hidden / kScaleBlock);
     for (int c0 = 0; c0 < count; c0 += 16) {
         const int c = c0 + fr < count ? c0 + fr : count - 1;
-        const uint8_t *x = static_cast<const uint8_t *>(p.x) + 2 * token_of[c] * p.ldx;
+        const uint8_t *x = static_cast<const uint8_t *>(p.x) + 2 * (token_of[c] * p.ldx + fg * 16);
         v4f ag = {0.f, 0.f, 0.f, 0.f}, au = {0.f, 0.f, 0.f, 0.f};
-        constexpr int U = 2;
-        for (int s0 = wave; s0 < steps; s0 += kWaves * U) {
+        // `mine` chooses and does not branch: loads would sink into the branches, one wait each
+        auto multiply = [&](const Codes &cg, const Codes &cu, const Halves &h, const float(&fgate)[S], const float(&fup)[S], bool mine) {
+            const v4f dg = block_product(cg, h), du = block_product(cu, h);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                ag[r] = mine ? __builtin_fmaf(dg[r], fgate[UNI ? 0 : r], ag[r]) : ag[r];
+                au[r] = mine ? __builtin_fmaf(du[r], fup[UNI ? 0 : r], au[r]) : au[r];
+            }
+        };
+        for (int s0 = wave; s0 < whole; s0 += NW * U) {
             Codes cg[U], cu[U];
             Halves h[U];
-            float fgate[U][UNI ? 1 : 4], fup[U][UNI ? 1 : 4];
+            float fgate[U][S], fup[U][S];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int s = s0 + u * kWaves;
-                if (s >= steps) break;
-                const int64_t k = (int64_t)s * kScaleBlock + fg * 16;
-                const bool whole = (int64_t)(s + 1) * kScaleBlock <= p.hidden;
-                cg[u] = load_codes(w_gate, k, p.hidden, whole);
-                cu[u] = load_codes(w_up, k, p.hidden, whole);
-                h[u] = load_halves(x, k, p.hidden, whole);
+            for (int u = 0; u < U; ++u) {  // beyond the last block: that one again, not added
+                const int64_t s = s0 + u * NW < whole ? s0 + u * NW : whole - 1;
+                cg[u] = load_codes(w_gate, s * kScaleBlock);
+                cu[u] = load_codes(w_up, s * kScaleBlock);
+                h[u] = load_halves(x, s * kScaleBlock);
 #pragma unroll
-                for (int r = 0; r < (UNI ? 1 : 4); ++r) {
+                for (int r = 0; r < S; ++r) {
                     fgate[u][r] = s_gate[r][s * p.up.s_blk];
                     fup[u][r] = s_up[r][s * p.up.s_blk];
                 }
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (s0 + u * kWaves >= steps) break;
-                const v4f dg = block_product(cg[u], h[u]), du = block_product(cu[u], h[u]);
+            for (int u = 0; u < U; ++u) multiply(turn(cg[u], scratch[wave], lane), turn(cu[u], scratch[wave], lane), h[u], fgate[u], fup[u], s0 + u * NW < whole);
+        }
+        if (p.hidden % kScaleBlock != 0 && wave == whole % NW) {  // the block that the rows end in
+            const int64_t k = (int64_t)whole * kScaleBlock, k_end = p.hidden - fg * 16;
+            float fgate[S], fup[S];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    ag[r] = __builtin_fmaf(dg[r], fgate[u][UNI ? 0 : r], ag[r]);
-                    au[r] = __builtin_fmaf(du[r], fup[u][UNI ? 0 : r], au[r]);
-                }
+            for (int r = 0; r < S; ++r) {
+                fgate[r] = s_gate[r][whole * p.up.s_blk];
+                fup[r] = s_up[r][whole * p.up.s_blk];
             }
+            const uint8_t *row = W + min64(i0 + fr, p.inner - 1) * p.up.ld + fg * 16;
+            multiply(load_last_codes(row, k, k_end, p.hidden >= 16), load_last_codes(row + to_up, k, k_end, p.hidden >= 16), load_last_halves(x, k, k_end, p.hidden >= 8), fgate, fup, true);
         }
         *reinterpret_cast<v4f *>(&part[wave][0][fr * 16 + fg * 4]) = ag;
         *reinterpret_cast<v4f *>(&part[wave][1][fr * 16 + fg * 4]) = au;
         __syncthreads();
-        if (t < 256) {  // (column, row)
-            const int col = c0 + (t >> 4), row = t & 15;
+        for (int q = t; q < 256; q += NW * 64) {  // (column, row)
+            const int col = c0 + (q >> 4), row = q & 15;
             float g = 0.f, u = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                g += part[w][0][t];
-                u += part[w][1][t];
+            for (int w = 0; w < NW; ++w) {
+                g += part[w][0][q];
+                u += part[w][1][q];
             }
             if (col < count && i0 + row < p.inner) {
                 const float h = g / (1.f + expf(-g)) * u * gate_of[col];
@@ -189,21 +186,22 @@ template <bool UNI> __global__ void __launch_bounds__(kWaves * 64) expert_up_ker
 // y for 16 of the hidden rows and all tokens: the waves share the picked experts (several waves an expert's contracted
 // blocks where there are few), add an expert's columns to their own LDS copy of the 16 x tokens result, and the
 // copies are summed in wave order: no atomics on values, the same bits on every run.
-__global__ void __launch_bounds__(kWaves * 64) expert_down_kernel(ExpertParams p, int k_parts)
+template <int NW, int U> __global__ void __launch_bounds__(NW * 64) expert_down_kernel(ExpertParams p, int k_parts)
 {
     extern __shared__ __attribute__((aligned(16))) float y_part[];  // [wave][token][16]
     __shared__ uint32_t bits[kExpertMaxExperts / 32];
     __shared__ int list[kExpertMaxPairs];
     __shared__ int listed;
-    __shared__ int columns[kWaves][64];
+    __shared__ int columns[NW][64];
+    __shared__ __attribute__((aligned(16))) uint8_t scratch[NW][2048];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int fr = lane & 15, fg = lane >> 4;
     const int64_t r0 = (int64_t)blockIdx.x * 16;
     const int per_wave = p.tokens * 16;
-    for (int i = t; i < kWaves * per_wave; i += kWaves * 64) y_part[i] = 0.f;
+    for (int i = t; i < NW * per_wave; i += NW * 64) y_part[i] = 0.f;
     if (t < kExpertMaxExperts / 32) bits[t] = 0;
     __syncthreads();
-    for (int i = t; i < p.tokens * p.top; i += kWaves * 64) {
+    for (int i = t; i < p.tokens * p.top; i += NW * 64) {
         const int e = p.pick[(i / p.top) * p.ld_pick + i % p.top];
         if (e >= 0 && e < p.experts) atomicOr(&bits[e >> 5], 1u << (e & 31));
     }
@@ -224,58 +222,64 @@ __global__ void __launch_bounds__(kWaves * 64) expert_down_kernel(ExpertParams p
     }
     const Picks picks = load_picks(p, lane);
     __syncthreads();
-    const int experts = listed, lanes = kWaves / k_parts;
-    const int part = wave / lanes, steps = (int)((p.inner + kScaleBlock - 1) / kScaleBlock);
-    const int64_t row = r0 + fr < p.hidden ? r0 + fr : p.hidden - 1;
-    float *mine = y_part + wave * per_wave;
+    const int experts = listed, lanes = NW / k_parts;
+    const int part = wave / lanes, whole = (int)(p.inner / kScaleBlock);
+    float *own_y = y_part + wave * per_wave;
+    const uint8_t *w0 = p.down.q + min64(r0 + (lane >> 2), p.hidden - 1) * p.down.ld + (lane & 3) * 16;
+    const uint8_t *last0 = p.down.q + min64(r0 + fr, p.hidden - 1) * p.down.ld + fg * 16;
+    const float *scale0 = p.down.scale + (r0 >> 7) * p.down.s_row;
+    const uint8_t *h0 = static_cast<const uint8_t *>(p.h) + 2 * fg * 16;
     for (int u = wave % lanes; u < experts; u += lanes) {
         const int e = __builtin_amdgcn_readfirstlane(list[u]);
+        const uint8_t *w = w0 + e * p.down.batch;
+        const float *scale = scale0 + e * p.down.s_batch;
         const int place = place_of(picks, e);
         const unsigned long long mask = __ballot(place >= 0);
         const int count = __popcll(mask);
         if (place >= 0) columns[wave][__popcll(mask & ((1ull << lane) - 1))] = lane * p.top + place;
         __builtin_amdgcn_wave_barrier();  // one wave's LDS accesses are in order
-        const uint8_t *w = p.down.q + e * p.down.batch + row * p.down.ld;
-        const float *S = p.down.scale + e * p.down.s_batch + (r0 >> 7) * p.down.s_row;
         for (int c0 = 0; c0 < count; c0 += 16) {
             const int pair = columns[wave][c0 + fr < count ? c0 + fr : count - 1];
-            const uint8_t *h = static_cast<const uint8_t *>(p.h) + 2 * pair * p.inner;
+            const uint8_t *h = h0 + 2 * pair * p.inner;
             v4f acc = {0.f, 0.f, 0.f, 0.f};
-            constexpr int U = 4;
-            for (int s0 = part; s0 < steps; s0 += k_parts * U) {
+            for (int s0 = part; s0 < whole; s0 += k_parts * U) {
                 Codes c[U];
                 Halves v[U];
                 float f[U];
 #pragma unroll
-                for (int q = 0; q < U; ++q) {
-                    const int s = s0 + q * k_parts;
-                    if (s >= steps) break;
-                    const int64_t k = (int64_t)s * kScaleBlock + fg * 16;
-                    const bool whole = (int64_t)(s + 1) * kScaleBlock <= p.inner;
-                    c[q] = load_codes(w, k, p.inner, whole);
-                    v[q] = load_halves(h, k, p.inner, whole);
-                    f[q] = S[s * p.down.s_blk];
+                for (int q = 0; q < U; ++q) {  // beyond the last block: that one again, not added
+                    const int64_t s = s0 + q * k_parts < whole ? s0 + q * k_parts : whole - 1;
+                    c[q] = load_codes(w, s * kScaleBlock);
+                    v[q] = load_halves(h, s * kScaleBlock);
+                    f[q] = scale[s * p.down.s_blk];
                 }
 #pragma unroll
-                for (int q = 0; q < U; ++q) {
-                    if (s0 + q * k_parts >= steps) break;
-                    const v4f d = block_product(c[q], v[q]);
+                for (int q = 0; q < U; ++q) {  // chosen, not branched over: loads would sink into the branches, one wait each
+                    const v4f d = block_product(turn(c[q], scratch[wave], lane), v[q]);
+                    const bool mine = s0 + q * k_parts < whole;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(d[r], f[q], acc[r]);
+                    for (int r = 0; r < 4; ++r) acc[r] = mine ? __builtin_fmaf(d[r], f[q], acc[r]) : acc[r];
                 }
             }
+            if (p.inner % kScaleBlock != 0 && part == whole % k_parts) {  // the block that the rows end in
+                const int64_t k = (int64_t)whole * kScaleBlock, k_end = p.inner - fg * 16;
+                const v4f d = block_product(load_last_codes(last0 + e * p.down.batch, k, k_end, p.inner >= 16), load_last_halves(h, k, k_end, p.inner >= 8));
+                const float f = scale[whole * p.down.s_blk];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(d[r], f, acc[r]);
+            }
             if (c0 + fr < count) {
-                v4f *dst = reinterpret_cast<v4f *>(mine + (pair / p.top) * 16 + fg * 4);
+                v4f *dst = reinterpret_cast<v4f *>(own_y + (pair / p.top) * 16 + fg * 4);
                 *dst += acc;
             }
         }
         __builtin_amdgcn_wave_barrier();
     }
     __syncthreads();
-    for (int i = t; i < per_wave; i += kWaves * 64) {
+    for (int i = t; i < per_wave; i += NW * 64) {
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) v += y_part[w * per_wave + i];
+        for (int w = 0; w < NW; ++w) v += y_part[w * per_wave + i];
         const int64_t r = r0 + (i & 15);
         if (r < p.hidden) static_cast<uint16_t *>(p.y)[(i >> 4) * p.ldy + r] = to_bf16(v);
     }
@@ -288,13 +292,20 @@ hipError_t launch_expert_layer(const ExpertParams &p, hipStream_t stream)
     const int pairs = p.tokens * p.top;
     const int by_pair = pairs < p.experts;
     const dim3 up((unsigned)((p.inner + 15) / 16), (unsigned)(by_pair ? pairs : p.experts));
-    if (p.inner % 16 == 0) hipLaunchKernelGGL((expert_up_kernel<true>), up, dim3(kWaves * 64), 0, stream, p, by_pair);
-    else hipLaunchKernelGGL((expert_up_kernel<false>), up, dim3(kWaves * 64), 0, stream, p, by_pair);
+    const bool uni = p.inner % 16 == 0;
+    if ((int64_t)up.x * up.y >= 2048) {
+        if (uni) hipLaunchKernelGGL((expert_up_kernel<true, 4, 2>), up, dim3(4 * 64), 0, stream, p, by_pair);
+        else hipLaunchKernelGGL((expert_up_kernel<false, 4, 2>), up, dim3(4 * 64), 0, stream, p, by_pair);
+    } else {
+        if (uni) hipLaunchKernelGGL((expert_up_kernel<true, 8, 1>), up, dim3(512), 0, stream, p, by_pair);
+        else hipLaunchKernelGGL((expert_up_kernel<false, 8, 1>), up, dim3(512), 0, stream, p, by_pair);
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // at most `pairs` experts: with fewer than eight, several waves share one expert's contracted blocks
-    const int k_parts = pairs >= 8 ? 1 : pairs >= 4 ? 2 : pairs >= 2 ? 4 : 8;
-    hipLaunchKernelGGL(expert_down_kernel, dim3((unsigned)((p.hidden + 15) / 16)), dim3(kWaves * 64), (size_t)kWaves * p.tokens * 16 * 4, stream, p, k_parts);
+    // at most `pairs` experts: with fewer than the waves, several waves share one expert's contracted blocks
+    int k_parts = 1;
+    while (k_parts < 8 && pairs * k_parts < 8) k_parts *= 2;
+    hipLaunchKernelGGL((expert_down_kernel<8, 2>), dim3((unsigned)((p.hidden + 15) / 16)), dim3(512), (size_t)8 * p.tokens * 16 * 4, stream, p, k_parts);
     return hipGetLastError();
 }
 

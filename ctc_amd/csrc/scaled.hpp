@@ -50,13 +50,13 @@ struct ScaledGemmParams {
 
 struct ScaledSchedule {
     int kind = 0;  // 0 skinny (no LDS staging), 1 the 128 tile, 2 the 256 tile
-    int waves = 8, split = 1;
+    int split = 1;
     size_t ws_bytes = 0;
 };
 // cus: compute units of the device; ws_limit: bytes of workspace the caller has
 ScaledSchedule schedule_scaled(const ScaledGemmParams &p, int cus, size_t ws_limit);
 hipError_t launch_scaled_gemm(ScaledGemmParams p, const ScaledSchedule &s, hipStream_t stream);
-hipError_t launch_scaled_skinny(const ScaledGemmParams &p, const ScaledSchedule &s, hipStream_t stream);
+hipError_t launch_scaled_skinny(const ScaledGemmParams &p, hipStream_t stream);
 
 // ---- the experts' layer for a few tokens (expert_kernels.hip) ----
 constexpr int kExpertMaxTokens = 64;

@@ -64,22 +64,30 @@ template <int FA, bool FAST, int NT> __device__ __forceinline__ void block_sums(
     }
 }
 
-// 16 bytes of a row from byte k on, zeros from byte k_end on; any alignment
-__device__ __forceinline__ uint4 load_chunk(const uint8_t *row, int64_t k, int64_t k_end)
+// 16 bytes of a row from byte k on, zeros from byte k_end on; any alignment.  Nothing behind k_end is read: a chunk that the
+// row ends in is the shifted end of the 16 bytes in front of k_end where the row has 16 (long_row), bytes otherwise.
+__device__ __forceinline__ uint4 load_chunk(const uint8_t *row, int64_t k, int64_t k_end, bool long_row)
 {
     uint4 u = make_uint4(0, 0, 0, 0);
-    if (k + 16 <= k_end) {
+    const int64_t left = k_end - k;
+    if (left >= 16) {
         __builtin_memcpy(&u, row + k, 16);
-    } else if (k < k_end) {
+    } else if (left > 0 && long_row) {
+        uint64_t w[2];
+        __builtin_memcpy(w, row + k_end - 16, 16);
+        const int bits = 8 * (16 - (int)left);  // 8 .. 120
+        const uint64_t lo = bits < 64 ? w[0] >> bits | w[1] << (64 - bits) : w[1] >> (bits - 64), hi = bits < 64 ? w[1] >> bits : 0;
+        u = make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+    } else if (left > 0) {
         uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (k + i < k_end) w[i >> 2] |= (uint32_t)row[k + i] << (8 * (i & 3));
+        for (int i = 0; i < 16; ++i) w[i >> 2] |= (i < left ? (uint32_t)row[k + (i < left ? i : 0)] : 0u) << (8 * (i & 3));
         u = make_uint4(w[0], w[1], w[2], w[3]);
     }
     return u;
 }
 
+__device__ __forceinline__ int64_t min64(int64_t a, int64_t b) { return a < b ? a : b; }
 __device__ __forceinline__ int64_t clamp_offset(int64_t o, int64_t hi) { return o < 0 ? 0 : (o > hi ? hi : o); }
 
 
@@ -121,6 +129,52 @@ __device__ __forceinline__ void store4(const ScaledGemmParams &p, int64_t at, in
 #pragma unroll
     for (int r = 0; r < 4; ++r)
         if (n + r < p.N) c[r] = to_bf16(p.alpha * v[r] + (p.beta != 0.f ? p.beta * from_bf16(c[r]) : 0.f));
+}
+
+// One block of 128 contracted elements of 16 rows of codes in a wave's registers, 32 bytes a lane.
+//
+// As the matrix core takes it, lane (fr = l % 16, fg = l / 16) holds bytes 16 fg .. and 64 + 16 fg .. of row fr.  Loaded that
+// way, sixteen neighbouring lanes touch sixteen rows and the L1's tag lookups, one per 16 bytes, bound the kernel at 4.4 TB/s.  So
+// the lanes load four abreast along a row (lane l: row l / 4, bytes 16 (l % 4) .. and 64 further: 64-byte pieces, a quarter of the
+// lookups), and `turn` passes the block through 2 KB of LDS that belong to the wave alone.
+//
+// The loads have no branch: those of several blocks stay in flight together, where a branch per block makes the compiler wait for each.
+struct Codes {
+    v4i lo, hi;
+};
+// row: the lane's row + 16 (l % 4)
+__device__ __forceinline__ Codes load_codes(const uint8_t *row, int64_t k)
+{
+    Codes c;
+    __builtin_memcpy(&c.lo, row + k, 16);
+    __builtin_memcpy(&c.hi, row + k + 64, 16);
+    return c;
+}
+__device__ __forceinline__ Codes turn(const Codes &c, uint8_t *scratch, int lane)
+{
+    // [half][row][four 16-byte chunks], chunk c of row r at c ^ (r / 4 & 3): rows four apart share their banks
+    const int wr = lane >> 2, wc = lane & 3, rr = lane & 15, rc = lane >> 4;
+    uint8_t *to = scratch + wr * 64 + ((wc ^ ((wr >> 2) & 3)) << 4);
+    const uint8_t *from = scratch + rr * 64 + ((rc ^ ((rr >> 2) & 3)) << 4);
+    *reinterpret_cast<v4i *>(to) = c.lo;
+    *reinterpret_cast<v4i *>(to + 1024) = c.hi;
+    // other lanes' bytes are read: one wave's LDS accesses complete in order, the compiler is kept from moving them
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    Codes o;
+    o.lo = *reinterpret_cast<const v4i *>(from);
+    o.hi = *reinterpret_cast<const v4i *>(from + 1024);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+    return o;
+}
+// the block that the rows end in, as the matrix core takes it (row: the lane's row fr + 16 fg, k_end counted from there): zeros from k_end on
+__device__ __forceinline__ Codes load_last_codes(const uint8_t *row, int64_t k, int64_t k_end, bool long_row)
+{
+    Codes c;
+    c.lo = __builtin_bit_cast(v4i, load_chunk(row, k, k_end, long_row));
+    c.hi = __builtin_bit_cast(v4i, load_chunk(row, k + 64, k_end, long_row));
+    return c;
 }
 
 }  // namespace scaled

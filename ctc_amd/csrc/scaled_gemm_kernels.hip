@@ -148,7 +148,7 @@ __device__ __forceinline__ void store_partial(float *w, int64_t left, v4f v, boo
 
 // BM x BN tile, WM x WN waves.  FA: A holds e5m2.  FAST: see BlockOperand.  BUNI: B's scale is one per 128 x 128 tile, hence
 // uniform in a wave.  DMA: both operands 16-byte aligned with row pitches that are multiples of 16: their blocks go
-// global -> LDS by DMA; otherwise every chunk passes through registers (byte-exact at any alignment).
+// global -> LDS by DMA; otherwise they pass through registers, requested a block ahead (byte-exact at any alignment).
 //
 // LDS, two stages of a block each: rows of 128 bytes, 16-byte chunk c of row r at c ^ (r / 2 & 7).  A fragment is the
 // chunks g and g + 4 of row l % 16 (g = l / 16), for both operands alike, so that the k order inside the MFMA's block
@@ -181,7 +181,6 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmP
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = wave / WN, wn = wave % WN;
     const int64_t a_entry = p.mode == kScaledDense ? it.entry : 0, b_entry = p.mode == kScaledContracted ? 0 : it.entry;
-    const int64_t steps = (it.k_end - it.k_begin + kScaleBlock - 1) / kScaleBlock;
     const int64_t blk0 = it.k_begin / kScaleBlock;
 
     // staging: thread t owns chunk slot t % 8 of rows t / 8 + i * T / 8; rows beyond the operand repeat its last one
@@ -206,7 +205,8 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmP
     const unsigned lds0 = lds_dma::lds_addr(image) + wave * 1024;
     const int64_t k_len = it.k_end - it.k_begin;
 
-    // stages the whole block s
+    uint4 held[DMA ? 1 : NA + NB];
+    // requests the whole block s
     auto stage = [&](int64_t s, int buf) {
         if constexpr (DMA) {
             const unsigned base = lds0 + buf * STAGE;
@@ -216,39 +216,24 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmP
             for (int i = 0; i < NB; ++i) lds_dma::dma16_split(B + s * kScaleBlock, b_off[i], base + BM * 128 + i * (T * 16));
         } else {
             const int64_t k = s * kScaleBlock + schunk * 16;
-            uint8_t *to = image + buf * STAGE + srow * 128 + slot * 16;
 #pragma unroll
-            for (int i = 0; i < NA; ++i) *reinterpret_cast<uint4 *>(to + i * (T * 16)) = load_chunk(A + a_row[i], k, k_len);
+            for (int i = 0; i < NA; ++i) __builtin_memcpy(&held[i], A + a_row[i] + k, 16);
 #pragma unroll
-            for (int i = 0; i < NB; ++i) *reinterpret_cast<uint4 *>(to + BM * 128 + i * (T * 16)) = load_chunk(B + b_row[i], k, k_len);
+            for (int i = 0; i < NB; ++i) __builtin_memcpy(&held[NA + i], B + b_row[i] + k, 16);
         }
     };
-    // the block that K ends in: the DMA takes its whole chunks (lanes beyond them fetch the start of their row instead: K is
-    // 16 or more), and behind the transfers' end those lanes write what belongs there, the rest of the row and zeros
-    const int64_t tail_left = k_len % kScaleBlock - schunk * 16;
-    auto stage_tail = [&](int64_t s, int buf) {
-        if constexpr (DMA) {
-            const unsigned base = lds0 + buf * STAGE;
-            const uint32_t k = tail_left >= 16 ? (uint32_t)(s * kScaleBlock) : 0u - schunk * 16;
+    // without DMA: the block that stage() requested, into LDS
+    auto put = [&](int buf) {
+        uint8_t *to = image + buf * STAGE + srow * 128 + slot * 16;
 #pragma unroll
-            for (int i = 0; i < NA; ++i) lds_dma::dma16_split(A, a_off[i] + k, base + i * (T * 16));
+        for (int i = 0; i < NA; ++i) *reinterpret_cast<uint4 *>(to + i * (T * 16)) = held[i];
 #pragma unroll
-            for (int i = 0; i < NB; ++i) lds_dma::dma16_split(B, b_off[i] + k, base + BM * 128 + i * (T * 16));
-        } else {
-            stage(s, buf);
-        }
+        for (int i = 0; i < NB; ++i) *reinterpret_cast<uint4 *>(to + BM * 128 + i * (T * 16)) = held[NA + i];
     };
-    auto mend_tail = [&](int64_t s, int buf) {
-        if constexpr (DMA) {
-            if (tail_left >= 16) return;
-            uint8_t *to = image + buf * STAGE + srow * 128 + slot * 16;
-            const int64_t k = s * kScaleBlock + schunk * 16;
-#pragma unroll 1
-            for (int i = 0; i < NA + NB; ++i) {
-                const uint8_t *row = i < NA ? A + (int64_t)min(srow + i * (T / 8), a_last) * p.a.ld : B + (int64_t)min(srow + (i - NA) * (T / 8), b_last) * p.b.ld;
-                *reinterpret_cast<uint4 *>(to + (i < NA ? i * (T * 16) : BM * 128 + (i - NA) * (T * 16))) = load_chunk(row, k, k_len);
-            }
-        }
+    // block s is in LDS when this has run in every wave
+    auto land = [&](int buf) {
+        if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else put(buf);
     };
     const int64_t whole = k_len / kScaleBlock;  // blocks in front of the one K ends in, if it ends in one
     // scales: thread t owns entry t of the tile's BM rows and BN columns
@@ -269,89 +254,104 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmP
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
 
-    if (steps > 0) {
-        const float v = *s_ptr;
-        s_ptr += s_step;
-        if (whole > 0) stage(0, 0);
-        else stage_tail(0, 0);
-        scales[t] = v;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (whole == 0) mend_tail(0, 0);
-        __syncthreads();
-    }
     // a wave whose rows all lie behind the last one only stages: a group's last tile with at most half of its rows takes half the time
     const bool active = it.m0 + wm * WTM < it.m_end;
     const int fr = lane & 15, fg = lane >> 4;
     // fragment addresses: row base + fr, chunks fg and fg + 4 under the row's swizzle (fr / 2 & 7: row bases are multiples of 16)
     const int sw = (fr >> 1) & 7;
     const int off0 = fr * 128 + ((fg ^ sw) << 4), off1 = fr * 128 + (((fg + 4) ^ sw) << 4);
+    // multiplies the block in stage `buf`
+    auto multiply = [&](int buf) {
+        const uint8_t *stage_base = image + buf * STAGE;
+        const uint8_t *ia0 = stage_base + wm * WTM * 128 + off0, *ia1 = stage_base + wm * WTM * 128 + off1;
+        const uint8_t *ib0 = stage_base + (BM + wn * WTN) * 128 + off0, *ib1 = stage_base + (BM + wn * WTN) * 128 + off1;
+        const float *fs = scales + buf * (BM + BN);
+        BlockOperand<0, FAST> fb[NT];
+        BlockOperand<FA, FAST> fa[2];
+        fa[0].set(*reinterpret_cast<const v4i *>(ia0), *reinterpret_cast<const v4i *>(ia1));
+#pragma unroll
+        for (int j = 0; j < NT; ++j) fb[j].set(*reinterpret_cast<const v4i *>(ib0 + j * 2048), *reinterpret_cast<const v4i *>(ib1 + j * 2048));
+        v4f sb[BUNI ? 1 : NT];
+        if constexpr (BUNI) {
+            sb[0][0] = fs[BM + wn * WTN];
+        } else {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) sb[j] = *reinterpret_cast<const v4f *>(fs + BM + wn * WTN + j * 16 + fg * 4);
+        }
+        float sa[MT];
+        sa[0] = fs[wm * WTM + fr];
+        v4f d[2][NT];
+        auto add = [&](int i, const v4f(&v)[NT], float f) {
+            if constexpr (BUNI) f *= sb[0][0];
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[j][r], BUNI ? f : f * sb[BUNI ? 0 : j][r], acc[i][j][r]);
+            // here and not where the sums are next used: the compiler would move the additions behind the whole block's MFMAs,
+            // with every tile's results live until then
+#pragma unroll
+            for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[i][j]));
+        };
+        if constexpr (!FAST) __builtin_amdgcn_s_setprio(1);  // (4 % here, nothing for the 8-bit form)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            if (i + 1 < MT) {
+                fa[(i + 1) & 1].set(*reinterpret_cast<const v4i *>(ia0 + (i + 1) * 2048), *reinterpret_cast<const v4i *>(ia1 + (i + 1) * 2048));
+                sa[i + 1] = fs[wm * WTM + (i + 1) * 16 + fr];
+            }
+            block_sums<FA, FAST, NT>(fb, fa[i & 1], d[i & 1]);
+            if (i > 0) add(i - 1, d[(i - 1) & 1], sa[i - 1]);
+            // one MFMA, then additions: a wave that waits for the matrix core has work, and the core always a request
+#pragma unroll
+            for (int j = 0; j < (FAST ? NT : 4 * NT); ++j) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, FAST ? (BUNI ? 5 : 8) : (BUNI ? 2 : 3), 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (!FAST) __builtin_amdgcn_s_setprio(0);
+        add(MT - 1, d[(MT - 1) & 1], sa[MT - 1]);
+    };
+    if (whole > 0) {
+        stage(0, 0);
+        scales[t] = *s_ptr;
+        land(0);
+        __syncthreads();
+    }
 #pragma unroll 1
-    for (int64_t s = 0; s < steps; ++s) {
+    for (int64_t s = 0; s < whole; ++s) {
         const int buf = (int)(s & 1);
-        const bool more = s + 1 < steps;
+        const bool more = s + 1 < whole;
         float s_next = 0.f;
         if (more) {
-            s_next = *s_ptr;
             s_ptr += s_step;
-            if (s + 1 < whole) stage(s + 1, buf ^ 1);
-            else stage_tail(s + 1, buf ^ 1);
+            s_next = *s_ptr;
+            stage(s + 1, buf ^ 1);
         }
-        if (active) {
-            const uint8_t *stage_base = image + buf * STAGE;
-            const uint8_t *ia0 = stage_base + wm * WTM * 128 + off0, *ia1 = stage_base + wm * WTM * 128 + off1;
-            const uint8_t *ib0 = stage_base + (BM + wn * WTN) * 128 + off0, *ib1 = stage_base + (BM + wn * WTN) * 128 + off1;
-            const float *fs = scales + buf * (BM + BN);
-            BlockOperand<0, FAST> fb[NT];
-            BlockOperand<FA, FAST> fa[2];
-            fa[0].set(*reinterpret_cast<const v4i *>(ia0), *reinterpret_cast<const v4i *>(ia1));
-#pragma unroll
-            for (int j = 0; j < NT; ++j) fb[j].set(*reinterpret_cast<const v4i *>(ib0 + j * 2048), *reinterpret_cast<const v4i *>(ib1 + j * 2048));
-            v4f sb[BUNI ? 1 : NT];
-            if constexpr (BUNI) {
-                sb[0][0] = fs[BM + wn * WTN];
-            } else {
-#pragma unroll
-                for (int j = 0; j < NT; ++j) sb[j] = *reinterpret_cast<const v4f *>(fs + BM + wn * WTN + j * 16 + fg * 4);
-            }
-            float sa[MT];
-            sa[0] = fs[wm * WTM + fr];
-            v4f d[2][NT];
-            auto add = [&](int i, const v4f(&v)[NT], float f) {
-                if constexpr (BUNI) f *= sb[0][0];
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[i][j][r] = __builtin_fmaf(v[j][r], BUNI ? f : f * sb[BUNI ? 0 : j][r], acc[i][j][r]);
-                // here and not where the sums are next used: the compiler would move the additions behind the whole block's MFMAs,
-                // with every tile's results live until then
-#pragma unroll
-                for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[i][j]));
-            };
-            if constexpr (!FAST) __builtin_amdgcn_s_setprio(1);  // (4 % here, nothing for the 8-bit form)
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                if (i + 1 < MT) {
-                    fa[(i + 1) & 1].set(*reinterpret_cast<const v4i *>(ia0 + (i + 1) * 2048), *reinterpret_cast<const v4i *>(ia1 + (i + 1) * 2048));
-                    sa[i + 1] = fs[wm * WTM + (i + 1) * 16 + fr];
-                }
-                block_sums<FA, FAST, NT>(fb, fa[i & 1], d[i & 1]);
-                if (i > 0) add(i - 1, d[(i - 1) & 1], sa[i - 1]);
-                // one MFMA, then additions: a wave that waits for the matrix core has work, and the core always a request
-#pragma unroll
-                for (int j = 0; j < (FAST ? NT : 4 * NT); ++j) {
-                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x2, FAST ? (BUNI ? 5 : 8) : (BUNI ? 2 : 3), 0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if constexpr (!FAST) __builtin_amdgcn_s_setprio(0);
-            add(MT - 1, d[(MT - 1) & 1], sa[MT - 1]);
-        }
+        if (active) multiply(buf);
         if (more) {
             scales[(buf ^ 1) * (BM + BN) + t] = s_next;
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (s + 1 == whole) mend_tail(s + 1, buf ^ 1);
+            land(buf ^ 1);
         }
+        __syncthreads();
+    }
+    // The block that K ends in, behind the loop (inside it, its branches cost the loop its registers): through registers, chunk
+    // by chunk, zeros beyond the end.
+    if (k_len % kScaleBlock != 0) {
+        const int buf = (int)(whole & 1);
+        if (whole > 0) s_ptr += s_step;
+        scales[buf * (BM + BN) + t] = *s_ptr;
+        uint8_t *to = image + buf * STAGE + srow * 128 + slot * 16;
+        const int64_t k = whole * kScaleBlock + schunk * 16;
+        const bool long_row = it.k_end >= 16;
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+            *reinterpret_cast<uint4 *>(to + i * (T * 16)) = load_chunk(A + (int64_t)min(srow + i * (T / 8), a_last) * p.a.ld, k, k_len, long_row);
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+            *reinterpret_cast<uint4 *>(to + BM * 128 + i * (T * 16)) = load_chunk(B + (int64_t)min(srow + i * (T / 8), b_last) * p.b.ld, k, k_len, long_row);
+        __syncthreads();
+        if (active) multiply(buf);
         __syncthreads();
     }
 
@@ -412,9 +412,13 @@ __global__ void __launch_bounds__(256) scaled_split_sum_kernel(ScaledGemmParams 
 
 template <int FA, bool FAST, bool BUNI> hipError_t launch_tiles(const ScaledGemmParams &p, int kind, bool dma, unsigned grid, hipStream_t stream)
 {
-    if (FAST && kind == 2)
-        hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 256, 256, 2, 4, true>), dim3(grid), dim3(512), 0, stream, p);
-    else if (dma)
+    if constexpr (FAST) {  // (two fragments of bf16 do not fit the registers beside 128 accumulators)
+        if (kind == 2) {
+            hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 256, 256, 2, 4, true>), dim3(grid), dim3(512), 0, stream, p);
+            return hipGetLastError();
+        }
+    }
+    if (dma)
         hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 128, 128, 2, 2, true>), dim3(grid), dim3(256), 0, stream, p);
     else
         hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 128, 128, 2, 2, false>), dim3(grid), dim3(256), 0, stream, p);

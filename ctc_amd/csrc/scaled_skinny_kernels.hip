@@ -14,27 +14,12 @@ using namespace scaled;
 
 namespace {
 
-struct Codes {
-    v4i lo, hi;
-};
-__device__ __forceinline__ Codes load_codes(const uint8_t *row, int64_t k, int64_t k_end, bool whole)
+// MT: row tiles of 16 in one pass; a group with more rows takes several passes over its part of B.  U: blocks in flight a wave
+template <int FA, bool BUNI, int MT, int NW, int U> __global__ void __launch_bounds__(NW * 64) scaled_skinny_kernel(ScaledGemmParams p)
 {
-    Codes c;
-    if (whole) {
-        __builtin_memcpy(&c.lo, row + k, 16);
-        __builtin_memcpy(&c.hi, row + k + 64, 16);
-    } else {
-        c.lo = __builtin_bit_cast(v4i, load_chunk(row, k, k_end));
-        c.hi = __builtin_bit_cast(v4i, load_chunk(row, k + 64, k_end));
-    }
-    return c;
-}
-
-// MT: row tiles of 16 in one pass; a group with more rows takes several passes over its part of B
-template <int FA, bool BUNI, int MT, int NW> __global__ void __launch_bounds__(NW * 64) scaled_skinny_kernel(ScaledGemmParams p)
-{
-    constexpr int U = MT == 1 ? 4 : 2;  // blocks in flight
+    constexpr int S = BUNI ? 1 : 4;
     __shared__ __attribute__((aligned(16))) float part[NW][MT * 256];
+    __shared__ __attribute__((aligned(16))) uint8_t scratch[NW][2048];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int fr = lane & 15, fg = lane >> 4;
     const int64_t entry = blockIdx.x / (unsigned)p.nbn, n0 = (int64_t)(blockIdx.x % (unsigned)p.nbn) * 16;
@@ -48,16 +33,17 @@ template <int FA, bool BUNI, int MT, int NW> __global__ void __launch_bounds__(N
         A += entry * p.a.batch;
         SA += entry * p.a.s_batch;
     }
-    const int64_t n_lane = n0 + fr < p.N ? n0 + fr : p.N - 1;
-    const uint8_t *b_row = p.b.q + entry * p.b.batch + n_lane * p.b.ld;
+    const uint8_t *B = p.b.q + entry * p.b.batch;
+    const int lr = lane >> 2, lc = (lane & 3) * 16;  // the row and the bytes that the lane loads
+    const uint8_t *b_row = B + min64(n0 + lr, p.N - 1) * p.b.ld + lc;
     const float *SB = p.b.scale + entry * p.b.s_batch;
-    const float *sb_ptr[BUNI ? 1 : 4];
+    const float *sb_ptr[S];
 #pragma unroll
-    for (int r = 0; r < (BUNI ? 1 : 4); ++r) {
+    for (int r = 0; r < S; ++r) {
         const int64_t n = BUNI ? n0 : n0 + fg * 4 + r;
         sb_ptr[r] = SB + ((n < p.N ? n : p.N - 1) >> p.b.shift) * p.b.s_row;
     }
-    const int steps = (int)((p.K + kScaleBlock - 1) / kScaleBlock);
+    const int whole = (int)(p.K / kScaleBlock);
     const int64_t c_entry = p.mode == kScaledRows ? 0 : entry * p.c_batch;
     const bool vec = ((p.ldc | p.c_batch) & 3) == 0 && (reinterpret_cast<uintptr_t>(p.C) & (p.c_f32 ? 15 : 7)) == 0;
 
@@ -66,50 +52,60 @@ template <int FA, bool BUNI, int MT, int NW> __global__ void __launch_bounds__(N
         const float *sa_ptr[MT];
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            int64_t m = m0 + i * 16 + fr;
-            m = m < m_end ? m : m_end - 1;
-            a_row[i] = A + m * p.a.ld;
-            sa_ptr[i] = SA + (m >> p.a.shift) * p.a.s_row;
+            a_row[i] = A + min64(m0 + i * 16 + lr, m_end - 1) * p.a.ld + lc;
+            sa_ptr[i] = SA + (min64(m0 + i * 16 + fr, m_end - 1) >> p.a.shift) * p.a.s_row;
         }
-        const int64_t rows = m_end - m0;
         v4f acc[MT];
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
-        for (int s0 = wave; s0 < steps; s0 += NW * U) {
-            Codes fb[U], fa[U][MT];
-            float sb[U][BUNI ? 1 : 4], sa[U][MT];
+        // `mine` chooses and does not branch: loads would sink into the branches, one wait each
+        auto multiply = [&](const Codes &cb, const Codes(&ca)[MT], const float(&sb)[S], const float(&sa)[MT], bool mine) {
+            BlockOperand<0, false> ob[1];
+            ob[0].set(cb.lo, cb.hi);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int s = s0 + u * NW;
-                if (s >= steps) break;
-                const int64_t k = (int64_t)s * kScaleBlock + fg * 16;
-                const bool whole = (int64_t)(s + 1) * kScaleBlock <= p.K;
-                fb[u] = load_codes(b_row, k, p.K, whole);
+            for (int i = 0; i < MT; ++i) {
+                BlockOperand<FA, false> oa;
+                oa.set(ca[i].lo, ca[i].hi);
+                v4f d[1];
+                block_sums<FA, false, 1>(ob, oa, d);
 #pragma unroll
-                for (int r = 0; r < (BUNI ? 1 : 4); ++r) sb[u][r] = sb_ptr[r][(int64_t)s * p.b.s_blk];
+                for (int r = 0; r < 4; ++r) acc[i][r] = mine ? __builtin_fmaf(d[0][r], sa[i] * sb[BUNI ? 0 : r], acc[i][r]) : acc[i][r];
+            }
+        };
+        for (int s0 = wave; s0 < whole; s0 += NW * U) {
+            Codes cb[U], ca[U][MT];
+            float sb[U][S], sa[U][MT];
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    if (i > 0 && rows <= i * 16) break;
-                    fa[u][i] = load_codes(a_row[i], k, p.K, whole);
-                    sa[u][i] = sa_ptr[i][(int64_t)s * p.a.s_blk];
-                }
+            for (int u = 0; u < U; ++u) {  // beyond the last block: that one again, not added
+                const int64_t s = s0 + u * NW < whole ? s0 + u * NW : whole - 1;
+                cb[u] = load_codes(b_row, s * kScaleBlock);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) ca[u][i] = load_codes(a_row[i], s * kScaleBlock);
+#pragma unroll
+                for (int r = 0; r < S; ++r) sb[u][r] = sb_ptr[r][s * p.b.s_blk];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) sa[u][i] = sa_ptr[i][s * p.a.s_blk];
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (s0 + u * NW >= steps) break;
-                BlockOperand<0, false> ob[1];
-                ob[0].set(fb[u].lo, fb[u].hi);
+                Codes tb = turn(cb[u], scratch[wave], lane), ta[MT];
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    if (i > 0 && rows <= i * 16) break;
-                    BlockOperand<FA, false> oa;
-                    oa.set(fa[u][i].lo, fa[u][i].hi);
-                    v4f d[1];
-                    block_sums<FA, false, 1>(ob, oa, d);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[i][r] = __builtin_fmaf(d[0][r], sa[u][i] * sb[u][BUNI ? 0 : r], acc[i][r]);
-                }
+                for (int i = 0; i < MT; ++i) ta[i] = turn(ca[u][i], scratch[wave], lane);
+                multiply(tb, ta, sb[u], sa[u], s0 + u * NW < whole);
             }
+        }
+        if (p.K % kScaleBlock != 0 && wave == whole % NW) {  // the block that K ends in
+            const int64_t k = (int64_t)whole * kScaleBlock;
+            Codes cb = load_last_codes(B + min64(n0 + fr, p.N - 1) * p.b.ld + fg * 16, k, p.K - fg * 16, p.K >= 16), ca[MT];
+            float sb[S], sa[MT];
+#pragma unroll
+            for (int r = 0; r < S; ++r) sb[r] = sb_ptr[r][whole * p.b.s_blk];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                ca[i] = load_last_codes(A + min64(m0 + i * 16 + fr, m_end - 1) * p.a.ld + fg * 16, k, p.K - fg * 16, p.K >= 16);
+                sa[i] = sa_ptr[i][whole * p.a.s_blk];
+            }
+            multiply(cb, ca, sb, sa, true);
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) *reinterpret_cast<v4f *>(&part[wave][(i * 16 + fr) * 16 + fg * 4]) = acc[i];
@@ -126,22 +122,17 @@ template <int FA, bool BUNI, int MT, int NW> __global__ void __launch_bounds__(N
     }
 }
 
-template <int FA, bool BUNI, int MT> void launch_rows(const ScaledGemmParams &p, int waves, unsigned grid, hipStream_t stream)
-{
-    if (waves == 16) hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, MT, 16>), dim3(grid), dim3(1024), 0, stream, p);
-    else if (waves == 8) hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, MT, 8>), dim3(grid), dim3(512), 0, stream, p);
-    else hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, MT, 4>), dim3(grid), dim3(256), 0, stream, p);
-}
-template <int FA, bool BUNI> void launch_b(const ScaledGemmParams &p, int waves, unsigned grid, hipStream_t stream)
+template <int FA, bool BUNI> void launch_b(const ScaledGemmParams &p, unsigned grid, hipStream_t stream)
 {
     const int64_t rows = p.mode == kScaledRows ? (p.M + p.batch - 1) / p.batch : p.M;
-    if (rows <= 16) launch_rows<FA, BUNI, 1>(p, waves, grid, stream);
-    else launch_rows<FA, BUNI, 2>(p, waves, grid, stream);
+    if (rows > 16) hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, 2, 8, 2>), dim3(grid), dim3(512), 0, stream, p);
+    else if (p.K <= 16 * kScaleBlock) hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, 1, 8, 2>), dim3(grid), dim3(512), 0, stream, p);
+    else hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, 1, 8, 4>), dim3(grid), dim3(512), 0, stream, p);
 }
 
 }  // namespace
 
-hipError_t launch_scaled_skinny(const ScaledGemmParams &pp, const ScaledSchedule &s, hipStream_t stream)
+hipError_t launch_scaled_skinny(const ScaledGemmParams &pp, hipStream_t stream)
 {
     ScaledGemmParams p = pp;
     p.nbn = (int)((p.N + 15) / 16);
@@ -149,11 +140,11 @@ hipError_t launch_scaled_skinny(const ScaledGemmParams &pp, const ScaledSchedule
     if (grid > 0x3fffff) return hipErrorInvalidValue;
     const bool uni = p.b.shift == 7;
     if (p.a.e5m2) {
-        if (uni) launch_b<1, true>(p, s.waves, (unsigned)grid, stream);
-        else launch_b<1, false>(p, s.waves, (unsigned)grid, stream);
+        if (uni) launch_b<1, true>(p, (unsigned)grid, stream);
+        else launch_b<1, false>(p, (unsigned)grid, stream);
     } else {
-        if (uni) launch_b<0, true>(p, s.waves, (unsigned)grid, stream);
-        else launch_b<0, false>(p, s.waves, (unsigned)grid, stream);
+        if (uni) launch_b<0, true>(p, (unsigned)grid, stream);
+        else launch_b<0, false>(p, (unsigned)grid, stream);
     }
     return hipGetLastError();
 }
