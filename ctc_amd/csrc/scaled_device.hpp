@@ -64,6 +64,12 @@ template <int FA, bool FAST, int NT> __device__ __forceinline__ void block_sums(
     }
 }
 
+__device__ __forceinline__ v4i load16(const uint8_t *q)  // any alignment
+{
+    v4i v;
+    __builtin_memcpy(&v, q, 16);
+    return v;
+}
 // 16 bytes of a row from byte k on, zeros from byte k_end on; any alignment.  Nothing behind k_end is read: a chunk that the
 // row ends in is the shifted end of the 16 bytes in front of k_end where the row has 16 (long_row), bytes otherwise.
 __device__ __forceinline__ uint4 load_chunk(const uint8_t *row, int64_t k, int64_t k_end, bool long_row)
@@ -146,8 +152,8 @@ struct Codes {
 __device__ __forceinline__ Codes load_codes(const uint8_t *row, int64_t k)
 {
     Codes c;
-    __builtin_memcpy(&c.lo, row + k, 16);
-    __builtin_memcpy(&c.hi, row + k + 64, 16);
+    c.lo = load16(row + k);
+    c.hi = load16(row + k + 64);
     return c;
 }
 __device__ __forceinline__ Codes turn(const Codes &c, uint8_t *scratch, int lane)

@@ -70,20 +70,21 @@ __device__ __forceinline__ int64_t count_group_tiles(const int32_t *offsets, int
     return n;
 }
 
-// XCD-contiguous runs of tile ids (workgroup i runs on XCD i % 8): neighbouring tiles share operand panels in one L2
-__device__ __forceinline__ int64_t xcd_run(int64_t id, int64_t total)
+// XCD-contiguous runs of tile ids (workgroup i runs on XCD i % 8): neighbouring tiles share operand panels in one L2.
+// Ids are below 2^23: 32-bit divisions, a fraction of the 64-bit ones' instructions.
+__device__ __forceinline__ uint32_t xcd_run(uint32_t id, uint32_t total)
 {
-    const int64_t q = total >> 3, r = total & 7, x = id & 7;
+    const uint32_t q = total >> 3, r = total & 7, x = id & 7;
     return x * q + (x < r ? x : r) + (id >> 3);
 }
 // tiles in groups of 8 tile rows, row index fastest: a run of ids covers a compact block of C
-__device__ __forceinline__ void grouped_order(int64_t id, int64_t nbm, int64_t nbn, int64_t &tm, int64_t &tn)
+__device__ __forceinline__ void grouped_order(uint32_t id, uint32_t nbm, uint32_t nbn, uint32_t &tm, uint32_t &tn)
 {
-    const int64_t per = 8 * nbn, g = id / per, first = g * 8;
-    const int64_t h = nbm - first < 8 ? nbm - first : 8;
-    const int64_t in = id - g * per;
-    tm = first + in % h;
+    const uint32_t per = 8 * nbn, g = id / per, first = g * 8;
+    const uint32_t h = nbm - first < 8 ? nbm - first : 8;
+    const uint32_t in = id - g * per;
     tn = in / h;
+    tm = first + in - tn * h;
 }
 
 // a value that is the same in all lanes, into scalar registers
@@ -95,31 +96,33 @@ __device__ __forceinline__ int64_t uniform(int64_t v)
 
 template <int BM, int BN> __device__ __forceinline__ bool find_item(const ScaledGemmParams &p, Item &it)
 {
-    int64_t id = blockIdx.x, tm, tn;
+    uint32_t id = blockIdx.x, tm, tn;
     it.chunk = 0;
     it.k_begin = 0;
     it.k_end = p.K;
     if (p.mode == kScaledRows) {
-        const int64_t rows = count_group_tiles(p.offsets, p.batch, p.M, BM);
-        const int64_t total = rows * p.nbn;
+        const uint32_t rows = __builtin_amdgcn_readfirstlane((int)count_group_tiles(p.offsets, p.batch, p.M, BM));
+        const uint32_t total = rows * (uint32_t)p.nbn;
         if (id >= total) return false;
         grouped_order(xcd_run(id, total), rows, p.nbn, tm, tn);
         int g = 0;
         if (!find_group_tile(p.offsets, p.batch, p.M, BM, tm, g, it.m0, it.m_end)) return false;
         it.entry = g;
-        it.n0 = tn * BN;
+        it.n0 = (int64_t)tn * BN;
         return true;
     }
-    const int64_t per_entry = (int64_t)p.nbm * p.nbn, total = per_entry * p.batch * p.split;
-    id = xcd_run(id, total);
-    it.entry = id / (per_entry * p.split);
-    id -= it.entry * per_entry * p.split;
-    it.chunk = (int)(id / per_entry);
-    id -= it.chunk * per_entry;
+    const uint32_t per_entry = (uint32_t)p.nbm * (uint32_t)p.nbn, per = per_entry * (uint32_t)p.split;
+    id = xcd_run(id, per * (uint32_t)p.batch);
+    const uint32_t entry = id / per;
+    id -= entry * per;
+    const uint32_t chunk = id / per_entry;
+    id -= chunk * per_entry;
+    it.entry = entry;
+    it.chunk = (int)chunk;
     grouped_order(id, p.nbm, p.nbn, tm, tn);
-    it.m0 = tm * BM;
+    it.n0 = (int64_t)tn * BN;
+    it.m0 = (int64_t)tm * BM;
     it.m_end = p.M;
-    it.n0 = tn * BN;
     if (p.mode == kScaledContracted) {
         // groups start at whole blocks; an offset that does not is taken at the block it falls into (the last one may be the ragged end of K)
         int64_t lo = clamp_offset(p.offsets[it.entry], p.K), hi = clamp_offset(p.offsets[it.entry + 1], p.K);
@@ -188,24 +191,19 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmP
     const uint8_t *A = p.a.q + a_entry * p.a.batch + it.m0 * p.a.ld + it.k_begin;
     const uint8_t *B = p.b.q + b_entry * p.b.batch + it.n0 * p.b.ld + it.k_begin;
     uint32_t a_off[NA], b_off[NB];  // from the tile's corner: at most 255 rows of at most 2^22 bytes where DMA is set
-    int64_t a_row[DMA ? 1 : NA], b_row[DMA ? 1 : NB];
     const int a_last = (int)((it.m_end - it.m0 < BM ? it.m_end - it.m0 : BM) - 1), b_last = (int)((p.N - it.n0 < BN ? p.N - it.n0 : BN) - 1);
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
-        const int r = min(srow + i * (T / 8), a_last);
-        if constexpr (DMA) a_off[i] = (uint32_t)r * (uint32_t)p.a.ld + schunk * 16;
-        else a_row[i] = r * p.a.ld;
+        a_off[i] = (uint32_t)min(srow + i * (T / 8), a_last) * (uint32_t)p.a.ld + schunk * 16;
     }
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-        const int r = min(srow + i * (T / 8), b_last);
-        if constexpr (DMA) b_off[i] = (uint32_t)r * (uint32_t)p.b.ld + schunk * 16;
-        else b_row[i] = r * p.b.ld;
+        b_off[i] = (uint32_t)min(srow + i * (T / 8), b_last) * (uint32_t)p.b.ld + schunk * 16;
     }
     const unsigned lds0 = lds_dma::lds_addr(image) + wave * 1024;
     const int64_t k_len = it.k_end - it.k_begin;
 
-    uint4 held[DMA ? 1 : NA + NB];
+    v4i held[DMA ? 1 : NA + NB];
     // requests the whole block s
     auto stage = [&](int64_t s, int buf) {
         if constexpr (DMA) {
@@ -217,18 +215,18 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmP
         } else {
             const int64_t k = s * kScaleBlock + schunk * 16;
 #pragma unroll
-            for (int i = 0; i < NA; ++i) __builtin_memcpy(&held[i], A + a_row[i] + k, 16);
+            for (int i = 0; i < NA; ++i) held[i] = load16(A + (int64_t)min(srow + i * (T / 8), a_last) * p.a.ld + k);
 #pragma unroll
-            for (int i = 0; i < NB; ++i) __builtin_memcpy(&held[NA + i], B + b_row[i] + k, 16);
+            for (int i = 0; i < NB; ++i) held[NA + i] = load16(B + (int64_t)min(srow + i * (T / 8), b_last) * p.b.ld + k);
         }
     };
     // without DMA: the block that stage() requested, into LDS
     auto put = [&](int buf) {
         uint8_t *to = image + buf * STAGE + srow * 128 + slot * 16;
 #pragma unroll
-        for (int i = 0; i < NA; ++i) *reinterpret_cast<uint4 *>(to + i * (T * 16)) = held[i];
+        for (int i = 0; i < NA; ++i) *reinterpret_cast<v4i *>(to + i * (T * 16)) = held[i];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) *reinterpret_cast<uint4 *>(to + BM * 128 + i * (T * 16)) = held[NA + i];
+        for (int i = 0; i < NB; ++i) *reinterpret_cast<v4i *>(to + BM * 128 + i * (T * 16)) = held[NA + i];
     };
     // block s is in LDS when this has run in every wave
     auto land = [&](int buf) {
@@ -364,6 +362,20 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmP
     float *ws = p.ws + ((int64_t)it.chunk * p.batch + it.entry) * p.M * p.N;
     const bool vec = p.split > 1 ? (p.N & 3) == 0
                                  : ((p.ldc | p.c_batch) & 3) == 0 && (reinterpret_cast<uintptr_t>(p.C) & (p.c_f32 ? 15 : 7)) == 0;
+    // f32: a lane's four columns are 16 bytes and a row's four lanes 64, whole sectors without the pass through LDS
+    if (vec && (p.N & 3) == 0 && (p.split > 1 || (p.c_f32 && p.beta == 0.f))) {
+        float *c = p.split > 1 ? ws : static_cast<float *>(p.C) + c_entry;
+        const int64_t ld = p.split > 1 ? p.N : p.ldc;
+        const float alpha = p.split > 1 ? 1.f : p.alpha;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const int64_t m = it.m0 + wm * WTM + i * 16 + fr, n = it.n0 + wn * WTN + fg * 4;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                if (m < it.m_end && n + j * 16 < p.N) *reinterpret_cast<v4f *>(c + m * ld + n + j * 16) = acc[i][j] * alpha;
+        }
+        return;
+    }
 #pragma unroll
     for (int h = 0; h < MT / 2; ++h) {
         if (h > 0) __syncthreads();
@@ -433,8 +445,11 @@ bool dma_ready(const ScaledMatrix &m, int64_t k) { return ((reinterpret_cast<uin
 ScaledSchedule schedule_scaled(const ScaledGemmParams &p, int cus, size_t ws_limit)
 {
     ScaledSchedule s;
-    const int64_t rows = p.mode == kScaledRows ? (p.M + p.batch - 1) / p.batch : p.M;
-    if (p.mode != kScaledContracted && rows <= 32) return s;
+    // Few rows: B is read for them alone, straight into registers.  Dense products up to 32 rows; groups up to a mean of 8, since
+    // shares are uneven and a group of more than 16 rows passes over its weights again (32 groups, weights 2048 x 4096:
+    // 54 us against 64 on the 128 tile at a mean of 8 rows, 73 against 67 at 12, 83 against 67 at 16).
+    if (p.mode == kScaledDense && p.M <= 32) return s;
+    if (p.mode == kScaledRows && p.M <= 8 * (int64_t)p.batch) return s;
     const int64_t entries = p.mode == kScaledRows ? 1 : p.batch;
     const auto tiles = [&](int64_t b) {
         const int64_t nbm = (p.M + b - 1) / b + (p.mode == kScaledRows ? p.batch / 2 : 0);

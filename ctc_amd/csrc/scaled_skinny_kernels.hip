@@ -1,11 +1,10 @@
 // Block-scaled 8-bit products with few rows of A (one token, or a few per expert): B is read once and is nearly all
 // there is to read, so the kernel is bound by HBM, or by latency where B is small.
 //
-// A workgroup owns 16 columns of C (rows of B); its waves take the blocks of 128 contracted elements in turn and hold the
-// operands in registers: the lanes of one load instruction cover 64 contiguous bytes of 16 rows, two instructions the
-// whole 128-byte block, and nothing passes through LDS before the waves' partial sums do (in wave order: the same
-// bits on every run).  Four blocks are in flight per wave: with eight waves 64 KB per CU, more than the 24 KB that
-// a microsecond of latency at 6 TB/s takes.
+// A workgroup owns 16 columns of C (rows of B); its waves take the blocks of 128 contracted elements in turn, two or four
+// in flight each, hold the operands in registers (turned through LDS of the wave's own: see Codes) and meet once, in the
+// sum of their partial results, in wave order: the same bits on every run.  1 x 131072 x 8192: 163 us, 6.6 TB/s; 16 rows x 131072 x
+// 4096: 114 us, 4.7 TB/s (A is as many bytes as B for every workgroup then, out of the L2).
 #include "scaled_device.hpp"
 
 namespace ctc {
@@ -122,12 +121,21 @@ template <int FA, bool BUNI, int MT, int NW, int U> __global__ void __launch_bou
     }
 }
 
+// Waves of a workgroup: two where there are workgroups enough and K is short (a wave then has eight blocks or more of its
+// own, and less of its life goes into starting and into the sum over the waves: 64 groups, 96 rows, 2048 x 2048 weights
+// 45 -> 32 us, 4096 x 1024 ones 80 -> 32), eight where there are few workgroups or K is long (1 x 4096 x 8192: 12 us against 17).
 template <int FA, bool BUNI> void launch_b(const ScaledGemmParams &p, unsigned grid, hipStream_t stream)
 {
     const int64_t rows = p.mode == kScaledRows ? (p.M + p.batch - 1) / p.batch : p.M;
-    if (rows > 16) hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, 2, 8, 2>), dim3(grid), dim3(512), 0, stream, p);
-    else if (p.K <= 16 * kScaleBlock) hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, 1, 8, 2>), dim3(grid), dim3(512), 0, stream, p);
-    else hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, 1, 8, 4>), dim3(grid), dim3(512), 0, stream, p);
+    const int64_t blocks = p.K / kScaleBlock;
+    const bool two = (grid >= 1024 && blocks <= 32) || (grid >= 512 && blocks <= 16);
+    if (rows > 16) {
+        if (two) hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, 2, 2, 2>), dim3(grid), dim3(128), 0, stream, p);
+        else hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, 2, 8, 2>), dim3(grid), dim3(512), 0, stream, p);
+    } else {
+        if (two) hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, 1, 2, 2>), dim3(grid), dim3(128), 0, stream, p);
+        else hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, 1, 8, 4>), dim3(grid), dim3(512), 0, stream, p);
+    }
 }
 
 }  // namespace

@@ -275,7 +275,7 @@ def test_groups_of_rows(cuda, counts, n, k, dtype):
     for e in range(len(counts)):
         if counts[e]:
             lo, hi = at[e], at[e + 1]
-            check_product(A[lo:hi], sa[lo:hi], B[e], sb[e], out[lo:hi], dtype, fast=rows > 32 * len(counts))
+            check_product(A[lo:hi], sa[lo:hi], B[e], sb[e], out[lo:hi], dtype, fast=rows > 8 * len(counts))
 
 
 @pytest.mark.parametrize("blocks", [("rows", "rows"), ("tiles", "tiles")])
