@@ -8,7 +8,9 @@
 // packed from the router's picks by one ballot (lane = token): a token that did not pick the expert is in no column, so
 // that nothing an expert's weights hold (NaN among it) reaches a token that did not pick it.
 // Between the kernels h = gate * silu(G x) * (U x) is rounded to bf16, as an activation between two layers is: the second
-// kernel's MFMA takes 16 bits, and every workgroup reads the whole h, half the bytes of f32.
+// kernel's MFMA takes 16 bits.  Its error in y is the size of y's own rounding (0.0024 of the norm together, 0.0017 alone).
+// Kept as two bf16 numbers, with two MFMAs, h costs as many bytes out of the L2 as the weights out of HBM: measured 116 us
+// against 80 for the second kernel of 32 tokens, 64 experts, 4096 x 1536.
 #include "scaled_device.hpp"
 
 namespace ctc {
