@@ -94,6 +94,21 @@ __device__ __forceinline__ int64_t uniform(int64_t v)
     return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
 }
 
+// The group that is `place` in the order of falling lengths (ties by index); beyond 64 groups, a wave's lanes, the order as it is
+__device__ __forceinline__ int longest_first(const int32_t *offsets, int groups, int64_t k, int place)
+{
+    if (groups > 64) return place;
+    const int lane = threadIdx.x & 63;
+    int len = -1;
+    if (lane < groups) len = (int)(clamp_offset(offsets[lane + 1], k) - clamp_offset(offsets[lane], k));
+    int rank = 0;
+    for (int j = 0; j < groups; ++j) {
+        const int other = __builtin_amdgcn_readlane(len, j);
+        rank += other > len || (other == len && j < lane);
+    }
+    return __ffsll((long long)__ballot(lane < groups && rank == place)) - 1;
+}
+
 template <int BM, int BN> __device__ __forceinline__ bool find_item(const ScaledGemmParams &p, Item &it)
 {
     uint32_t id = blockIdx.x, tm, tn;
@@ -112,12 +127,16 @@ template <int BM, int BN> __device__ __forceinline__ bool find_item(const Scaled
         return true;
     }
     const uint32_t per_entry = (uint32_t)p.nbm * (uint32_t)p.nbn, per = per_entry * (uint32_t)p.split;
-    id = xcd_run(id, per * (uint32_t)p.batch);
+    // Groups of the contracted index differ in length: each is spread over all XCDs, and the longest come first.  Entries of a
+    // batch are equal and stay together.
+    const bool spread = p.mode == kScaledContracted;
+    if (!spread) id = xcd_run(id, per * (uint32_t)p.batch);
     const uint32_t entry = id / per;
     id -= entry * per;
+    if (spread) id = xcd_run(id, per);
     const uint32_t chunk = id / per_entry;
     id -= chunk * per_entry;
-    it.entry = entry;
+    it.entry = spread ? longest_first(p.offsets, p.batch, p.K, (int)entry) : (int)entry;
     it.chunk = (int)chunk;
     grouped_order(id, p.nbm, p.nbn, tm, tn);
     it.n0 = (int64_t)tn * BN;
