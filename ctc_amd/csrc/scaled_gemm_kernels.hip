@@ -477,8 +477,11 @@ ScaledSchedule schedule_scaled(const ScaledGemmParams &p, int cus, size_t ws_lim
     s.kind = !p.c_f32 && dma_ready(p.a, p.K) && dma_ready(p.b, p.K) && tiles(256) >= cus * 3 / 4 ? 2 : 1;
     if (s.kind == 1 && p.mode == kScaledDense && tiles(128) < cus) {
         const int64_t steps = (p.K + kScaleBlock - 1) / kScaleBlock;
+        // chunks of eight blocks or more, 64 at most: a second launch has to pay (150 x 260 x 16384: 20 us in chunks of four, 16 of
+        // eight, 18 of sixteen, 84 whole; 128 x 128 x 131072: 80 in 256 chunks, 47 in 128, 35 in 64, 614 whole)
         int64_t split = 2 * cus / tiles(128);
-        if (split > steps / 4) split = steps / 4;
+        if (split > steps / 8) split = steps / 8;
+        if (split > 64) split = 64;
         const size_t one = (size_t)p.M * p.N * p.batch * 4;
         if (split > 1 && (size_t)split * one > ws_limit) split = (int64_t)(ws_limit / one);
         if (split > 1) {
