@@ -6,6 +6,7 @@
 #include <atomic>
 #include <cstring>
 #include <string>
+#include <utility>
 
 #include "api_internal.hpp"
 #include "scaled.hpp"
@@ -17,6 +18,12 @@ using ctc_internal::set_last_hip_error;
 
 std::atomic<int64_t> g_skinny{0}, g_tile128{0}, g_tile256{0}, g_split{0};
 
+// elements that an operand may span: offsets, in bytes as well, stay far inside 64 bits
+constexpr double kMaxSpan = 70368744177664.0;  // 2^46
+double span(int64_t batch, int64_t batch_stride, int64_t rows, int64_t ld, int64_t cols)
+{
+    return (double)(batch - 1) * (double)batch_stride + (double)(rows - 1) * (double)ld + (double)cols;
+}
 constexpr int64_t kMaxDim = 0x7fffffff - 4096;  // row, column and block indexes are 32-bit inside a launch
 
 int refuse(const char *what, const char *why) { return set_last_error(CTC_TC_EINVAL, std::string(what) + ": " + why); }
@@ -71,7 +78,42 @@ int check_matrix(const char *what, const char *name, const ctc_tc_scaled_matrix 
     if (m->ld < cols) return set_last_error(CTC_TC_EINVAL, w + " has a leading dimension below its row length");
     if (m->batch_stride < 0 || m->scale_row < 0 || m->scale_block < 0 || m->scale_batch < 0)
         return set_last_error(CTC_TC_EINVAL, w + " has a negative stride");
+    if (span(batch, m->batch_stride, rows, m->ld, cols) > kMaxSpan ||
+        span(batch, m->scale_batch, rows, m->scale_row, 1) + (double)blocks_of(cols) * (double)m->scale_block > kMaxSpan)
+        return set_last_error(CTC_TC_EUNSUPPORTED, w + " spans too much memory");
     return CTC_TC_OK;
+}
+
+// `batch` matrices of rows x cols at these strides that would write to the same place: neither whole matrices nor the
+// matrices' rows (a batch index between the two) stand apart
+bool overlap(int64_t rows, int64_t cols, int64_t ld, int64_t batch, int64_t stride)
+{
+    if (batch <= 1) return false;
+    const bool whole = (double)stride >= span(1, 0, rows, ld, cols);
+    const bool between = stride >= cols && (rows <= 1 || (double)ld >= span(1, 0, batch, stride, cols));
+    return !whole && !between;
+}
+
+// a matrix that the quantiser writes: nothing of it twice
+int check_written(const char *what, const char *name, const ctc_tc_scaled_matrix &m, int64_t rows, int64_t cols, int64_t batch)
+{
+    const int64_t r = m.block == CTC_TC_BLOCK_TILES ? blocks_of(rows) : rows, c = blocks_of(cols);
+    // the scales' three strides in rising order, each past the extent of those below it
+    int64_t stride[3] = {m.scale_row, m.scale_block, m.scale_batch}, n[3] = {r, c, batch};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (stride[j] < stride[i]) {
+                std::swap(stride[i], stride[j]);
+                std::swap(n[i], n[j]);
+            }
+    double extent = 1;
+    bool twice = overlap(rows, cols, m.ld, batch, m.batch_stride);
+    for (int i = 0; i < 3; ++i) {
+        if (n[i] == 1) continue;
+        twice = twice || (double)stride[i] < extent;
+        extent += (double)(n[i] - 1) * (double)stride[i];
+    }
+    return twice ? set_last_error(CTC_TC_EINVAL, std::string(what) + ": " + name + " overlaps itself") : CTC_TC_OK;
 }
 
 int check_result(const char *what, const void *C, int64_t ldc, int64_t c_batch, int64_t rows, int64_t n, int64_t batch, int dtype)
@@ -81,7 +123,9 @@ int check_result(const char *what, const void *C, int64_t ldc, int64_t c_batch, 
     if (!C) return refuse(what, "the result is null");
     if (reinterpret_cast<uintptr_t>(C) & (dtype == CTC_TC_F32 ? 3 : 1)) return set_last_error(CTC_TC_EALIGN, std::string(what) + ": the result is not aligned to its elements");
     if (ldc < n) return refuse(what, "the result's leading dimension is below its row length");
-    if (batch > 1 && c_batch < (rows - 1) * ldc + n) return refuse(what, "the result's matrices overlap");
+    if (batch > 1 && c_batch < 0) return refuse(what, "a stride of the result is negative");
+    if (span(batch, batch > 1 ? c_batch : 0, rows, ldc, n) > kMaxSpan) return unsupported(what, "the result spans too much memory");
+    if (overlap(rows, n, ldc, batch, c_batch)) return refuse(what, "the result's matrices overlap");
     return CTC_TC_OK;
 }
 
@@ -132,6 +176,13 @@ int ctc_tc_block_quantize(const void *x, int64_t rows, int64_t cols, int64_t ldx
     if (!x) return refuse(what, "the input is null");
     if (reinterpret_cast<uintptr_t>(x) & (src_dtype == CTC_TC_F32 ? 3 : 1)) return set_last_error(CTC_TC_EALIGN, "block_quantize: the input is not aligned to its elements");
     if (ldx < cols || batch_stride_x < 0) return refuse(what, "the input's leading dimension is below its row length, or a stride is negative");
+    if (span(batch, batch_stride_x, rows, ldx, cols) > kMaxSpan) return unsupported(what, "the input spans too much memory");
+    if (out) {
+        if (int rc = check_written(what, "the result", *out, rows, cols, batch)) return rc;
+    }
+    if (out_t) {
+        if (int rc = check_written(what, "the transposed result", *out_t, cols, rows, batch)) return rc;
+    }
     if (rows > kMaxDim || cols > kMaxDim || batch > 65535 || blocks_of(rows) * blocks_of(cols) > (1 << 23)) return unsupported(what, "too large for one launch");
     ctc::QuantizeParams p;
     p.x = x;

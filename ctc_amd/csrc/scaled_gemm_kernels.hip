@@ -470,16 +470,16 @@ ScaledSchedule schedule_scaled(const ScaledGemmParams &p, int cus, size_t ws_lim
     if (p.mode == kScaledDense && p.M <= 32) return s;
     if (p.mode == kScaledRows && p.M <= 8 * (int64_t)p.batch) return s;
     const int64_t entries = p.mode == kScaledRows ? 1 : p.batch;
-    const auto tiles = [&](int64_t b) {
+    const auto tiles = [&](int64_t b) -> double {  // (the product of three 31-bit counts)
         const int64_t nbm = (p.M + b - 1) / b + (p.mode == kScaledRows ? p.batch / 2 : 0);
-        return nbm * ((p.N + b - 1) / b) * entries;
+        return (double)nbm * (double)((p.N + b - 1) / b) * (double)entries;
     };
     s.kind = !p.c_f32 && dma_ready(p.a, p.K) && dma_ready(p.b, p.K) && tiles(256) >= cus * 3 / 4 ? 2 : 1;
     if (s.kind == 1 && p.mode == kScaledDense && tiles(128) < cus) {
         const int64_t steps = (p.K + kScaleBlock - 1) / kScaleBlock;
         // chunks of eight blocks or more, 64 at most: a second launch has to pay (150 x 260 x 16384: 20 us in chunks of four, 16 of
         // eight, 18 of sixteen, 84 whole; 128 x 128 x 131072: 80 in 256 chunks, 47 in 128, 35 in 64, 614 whole)
-        int64_t split = 2 * cus / tiles(128);
+        int64_t split = (int64_t)(2 * cus / tiles(128));
         if (split > steps / 8) split = steps / 8;
         if (split > 64) split = 64;
         const size_t one = (size_t)p.M * p.N * p.batch * 4;
@@ -501,16 +501,17 @@ hipError_t launch_scaled_gemm(ScaledGemmParams p, const ScaledSchedule &s, hipSt
     p.split = s.split;
     const int64_t steps = (p.K + kScaleBlock - 1) / kScaleBlock;
     p.steps_per = (int)((steps + s.split - 1) / s.split);
-    int64_t grid = (int64_t)p.nbm * p.nbn * p.batch * p.split;
+    double count = (double)p.nbm * p.nbn * p.batch * p.split;
     // row tiles of ragged groups: each group adds at most one partly filled tile
-    if (p.mode == kScaledRows) grid = (p.M / b + (p.batch < p.M ? p.batch : p.M)) * (int64_t)p.nbn;
-    if (grid > 0x7fffff) return hipErrorInvalidValue;
+    if (p.mode == kScaledRows) count = (double)(p.M / b + (p.batch < p.M ? p.batch : p.M)) * p.nbn;
+    if (count > 0x7fffff) return hipErrorInvalidValue;
+    const unsigned grid = (unsigned)count;
     const bool uni = p.b.shift == 7, dma = dma_ready(p.a, p.K) && dma_ready(p.b, p.K);
     const bool fast = !p.c_f32;  // an f32 result takes f32 sums (see block_sums)
     typedef hipError_t (*launcher)(const ScaledGemmParams &, int, bool, unsigned, hipStream_t);
     static const launcher table[2][2][2] = {{{launch_tiles<0, false, false>, launch_tiles<0, false, true>}, {launch_tiles<0, true, false>, launch_tiles<0, true, true>}},
                                             {{launch_tiles<1, false, false>, launch_tiles<1, false, true>}, {launch_tiles<1, true, false>, launch_tiles<1, true, true>}}};
-    const hipError_t e = table[p.a.e5m2][fast][uni](p, s.kind, dma, (unsigned)grid, stream);
+    const hipError_t e = table[p.a.e5m2][fast][uni](p, s.kind, dma, grid, stream);
     if (e != hipSuccess || p.split == 1) return e;
     int64_t blocks = (((p.N + 3) >> 2) * p.M * p.batch + 255) / 256;
     if (blocks > 256 * 16) blocks = 256 * 16;

@@ -170,7 +170,7 @@ def block_quantize(x, block="rows", dtype=None, transposed=False, out=None, stre
     ldx = _pitch("x", shape, stride)
     rows, cols = shape[-2:]
     lead = shape[:-2]
-    plain, turned = transposed is not True, transposed is not False
+    plain, turned = transposed == "both" or not transposed, bool(transposed)
     given = None
     if out is not None:
         given = tuple(out)
@@ -227,7 +227,7 @@ def scaled_contract(A, scale_a, B, scale_b, out=None, dtype=None, alpha=1.0, bet
         # (32: products of so few rows never split)
         room = check(st.lib.ctc_tc_scaled_workspace_bytes(m, n, k, batch)) if m > 32 else 0
         ws = st.empty(room, dtype=st.torch.uint8, device=device) if room else None
-        check(st.lib.ctc_tc_scaled_contract(m, n, k, batch, _byref(a), _byref(b), alpha, beta, c.data_ptr(), ldc, stride, code,
+        check(st.lib.ctc_tc_scaled_contract(m, n, k, batch, _byref(a), _byref(b), float(alpha), float(beta), c.data_ptr(), ldc, stride, code,
                                             ws.data_ptr() if room else None, room, raw))
         return c
 
@@ -266,7 +266,7 @@ def scaled_grouped_contract(A, scale_a, B, scale_b, offsets, along="rows", out=N
     def call(raw):
         c, code, ldc, stride = _result(st, out, (m, n) if rows else (groups, m, n), dtype or st.bf16, device)
         check(st.lib.ctc_tc_scaled_grouped_contract(GROUPS_ROWS if rows else GROUPS_CONTRACTED, groups, offsets.data_ptr(), m, n, k, _byref(a),
-                                                    _byref(b), alpha, beta, c.data_ptr(), ldc, stride, code, raw))
+                                                    _byref(b), float(alpha), float(beta), c.data_ptr(), ldc, stride, code, raw))
         return c
 
     return _run(st, device, stream, call)

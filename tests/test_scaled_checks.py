@@ -47,7 +47,10 @@ def experts(tokens=2, top=2, experts=8, hidden=256, inner=256, x=ADDR, ldx=256, 
     (dict(out=matrix(q=None)), EINVAL), (dict(out=matrix(scale=None)), EINVAL), (dict(out=matrix(scale=ADDR + 2)), EALIGN),
     (dict(out=matrix(ld=255)), EINVAL), (dict(out=matrix(dtype=_lib.BF16)), EINVAL), (dict(out=matrix(block=2)), EINVAL),
     (dict(out=matrix(s_row=-1)), EINVAL), (dict(out_t=matrix(ld=7)), EINVAL), (dict(out_t=matrix(dtype=_lib.F8E5M2)), EINVAL),
-    (dict(out_t=TILES), EINVAL), (dict(batch=1 << 17), EUNSUPPORTED), (dict(rows=1 << 31), EUNSUPPORTED), (dict(stride=-1), EINVAL),
+    (dict(out_t=TILES), EINVAL), (dict(batch=1 << 17, out=matrix(batch=1 << 20, s_batch=1 << 20)), EUNSUPPORTED), (dict(rows=1 << 31), EINVAL), (dict(stride=-1), EINVAL),
+    # results that would be written twice: scales of all rows, of both blocks, of both matrices, codes of both matrices
+    (dict(out=matrix(s_row=0)), EINVAL), (dict(out=matrix(s_blk=4)), EINVAL), (dict(batch=2, out=matrix(batch=8 * 256)), EINVAL),
+    (dict(batch=2, out=matrix(s_batch=128)), EINVAL), (dict(out=matrix(ld=1 << 50)), EUNSUPPORTED), (dict(ldx=1 << 50), EUNSUPPORTED),
 ])
 def test_quantizer_refuses(kw, code):
     assert quantize(**kw) == code
@@ -59,7 +62,11 @@ def test_quantizer_refuses(kw, code):
     (dict(a=matrix(dtype=_lib.BF16)), EINVAL), (dict(b=matrix(dtype=_lib.F8E5M2)), EUNSUPPORTED), (dict(a=matrix(ld=255)), EINVAL),
     (dict(b=matrix(q=None)), EINVAL), (dict(b=matrix(scale=ADDR + 1)), EALIGN), (dict(C=None), EINVAL), (dict(ldc=63), EINVAL),
     (dict(dtype=_lib.F64), EUNSUPPORTED), (dict(dtype=_lib.F8E4M3), EUNSUPPORTED), (dict(C=ADDR + 1), EALIGN), (dict(dtype=_lib.F32, C=ADDR + 2), EALIGN),
-    (dict(batch=2, stride=64), EINVAL), (dict(ws=ADDR + 8, room=64), EALIGN), (dict(room=-1), EINVAL),
+    (dict(batch=2, stride=64), EINVAL), (dict(ws=ADDR + 8, room=64), EALIGN), (dict(room=-1), EINVAL), (dict(a=matrix(ld=1 << 50)), EUNSUPPORTED),
+    (dict(ldc=1 << 50), EUNSUPPORTED), (dict(batch=2, stride=-64 * 64), EINVAL),
+    # more tiles than a launch takes, and than 64 bits count
+    (dict(m=1 << 23, n=1 << 23, ldc=1 << 23, b=matrix(s_blk=1 << 23), a=matrix(s_blk=1 << 23)), EUNSUPPORTED),
+    (dict(m=1 << 30, n=1 << 30, batch=65535, ldc=1 << 30, a=matrix(ld=256), b=matrix(ld=256), stride=1 << 60), EUNSUPPORTED),
 ])
 def test_product_refuses(kw, code):
     assert product(**kw) == code
@@ -84,6 +91,52 @@ def test_grouped_product_refuses(kw, code):
 def test_expert_layer_refuses(kw, code):
     assert experts(**kw) == code
     assert b"expert_layer" in _lib.load().ctc_tc_last_error()
+
+
+def test_quantizer_takes_every_order_of_a_results_indexes():
+    """[rows, batch, columns] in memory, scales with the batch fastest: nothing overlaps (no rows, so nothing is launched)."""
+    L = _lib.load()
+    m = matrix(ld=3 * 256, batch=256, s_row=3, s_blk=3 * 8, s_batch=1)
+    assert L.ctc_tc_block_quantize(None, 8, 256, 256, 3, 8 * 256, _lib.BF16, ref(m), None, None) == EINVAL
+    assert b"input is null" in L.ctc_tc_last_error()
+    assert quantize(batch=3, stride=8 * 256, x=None, out=m) == EINVAL
+
+
+def test_kernels_that_set_m0_from_assembly_have_no_other_m0_user(tmp_path):
+    """The block-scaled products' LDS-DMA transfers overwrite M0 in inline assembly, which cannot be declared: in their code
+    every instruction that names M0 must be the move in front of a transfer, and every transfer have one."""
+    import os
+    import re
+    import shutil
+    import subprocess
+    objdump = "/opt/rocm/lib/llvm/bin/llvm-objdump"
+    if not os.path.exists(objdump):
+        pytest.skip("llvm-objdump is not installed")
+    lib = tmp_path / "libctc_tc.so"
+    shutil.copy(_lib.LIB_PATH, lib)
+    subprocess.run([objdump, "--offloading", str(lib)], check=True, capture_output=True, cwd=tmp_path)
+    name, last, kernels = None, "", {}
+    for obj in (p for p in tmp_path.iterdir() if "amdgcn" in p.name and p.stat().st_size > 0):
+        text = subprocess.run([objdump, "-d", "--no-show-raw-insn", str(obj)], check=True, capture_output=True, text=True).stdout
+        if "scaled_gemm_kernel" not in text:
+            continue
+        for line in text.splitlines():
+            m = re.match(r"^[0-9a-f]+ <(\S+)>:", line)
+            if m:
+                name = m.group(1) if "scaled_gemm_kernel" in m.group(1) else None
+                continue
+            inst = re.sub(r"\s*//.*$", "", line).strip()
+            if name is None or not inst:
+                continue
+            assert not re.match(r"(v_movrel|s_movrel|s_sendmsg|v_interp|ds_gws|v_pk_(add|mul|fma)_f32)", inst), (name, inst)
+            if inst.startswith("global_load_lds"):
+                kernels[name] = kernels.get(name, 0) + 1
+                assert re.match(r"s_mov_b32 m0, s\d+$", last), (name, last, inst)
+            else:
+                assert not re.match(r"s_mov_b32 m0", last), (name, last, inst)
+                assert "m0" not in inst or re.match(r"s_mov_b32 m0, s\d+$", inst), (name, inst)
+            last = inst
+    assert len(kernels) == 12, kernels  # two types of A, two of scales: three tiles with DMA (two sums on the small one)
 
 
 def test_nothing_to_do_succeeds_without_a_device():

@@ -50,6 +50,7 @@ def test_quantizer(cuda, block, dtype, src, shape):
     same_codes(qt, wqt)
     assert torch.equal(s.cpu(), ws) and torch.equal(st.cpu(), wst)
     assert torch.equal(ctc_amd.block_quantize(x, block, dtype)[0].cpu().view(torch.uint8), q.cpu().view(torch.uint8))
+    assert len(ctc_amd.block_quantize(x, block, dtype, transposed=1)) == 2
     one = ctc_amd.block_quantize(x, block, dtype, transposed=True)
     same_codes(one[0], wqt)
     assert torch.equal(one[1].cpu(), wst)
@@ -248,6 +249,52 @@ def test_operands_with_strided_scales_and_a_shared_batch(cuda):
     check_product(A, sa, torch.stack([B.view(torch.uint8)] * 2).view(E4M3), torch.stack([sb, sb]), got, F32)
 
 
+def far(rows, cols, pitch, dtype, values):
+    """A rows x cols view whose rows lie `pitch` elements apart: the last one starts beyond 2^32 bytes."""
+    assert (rows - 1) * pitch * values.element_size() > 2 ** 32
+    t = torch.empty((rows - 1) * pitch + cols, dtype=dtype, device="cuda")
+    v = t.as_strided((rows, cols), (pitch, 1))
+    v.copy_(values)
+    return v
+
+
+@pytest.mark.parametrize("m", [3, 150])
+@pytest.mark.parametrize("pitch", [1 << 22, (1 << 22) + 16, (1 << 22) + 1])
+def test_operands_and_results_beyond_32_bit_offsets(cuda, m, pitch):
+    """The DMA's 32-bit offsets end at pitches of 2^22: beyond, and at odd ones, the blocks pass through registers."""
+    g = gen(14)
+    A, sa = ref.random_operand(g, (m, 300), "rows")
+    B, sb = ref.random_operand(g, (1100, 300), "tiles")
+    wide = far(1100, 300, pitch, torch.uint8, B.view(torch.uint8)).view(E4M3)
+    check_product(A, sa, B, sb, ctc_amd.scaled_contract(A, sa, wide, sb), BF16)
+    out = far(1100, m, 1 << 20, F32, torch.zeros(1100, m, device="cuda"))
+    ctc_amd.scaled_contract(wide, sb, A, sa, out=out)
+    check_product(B, sb, A, sa, out, F32)
+
+
+def test_quantizer_beyond_32_bit_offsets(cuda):
+    x = torch.randn(1100, 200, generator=gen(15))
+    wide = far(1100, 200, 1 << 20, F32, x.cuda())
+    q, s, qt, st = ctc_amd.block_quantize(wide, transposed="both")
+    wq, ws = ref.quantize(x, "rows", E4M3)
+    same_codes(q, wq)
+    assert torch.equal(s.cpu(), ws)
+    same_codes(qt, ref.quantize(x.t(), "rows", E4M3)[0])
+
+
+@pytest.mark.parametrize("m", [5, 140])
+def test_product_with_the_batch_between_rows_and_columns(cuda, m):
+    g = gen(16)
+    A, sa = ref.random_operand(g, (m, 3, 256), "rows")  # [m, batch, k]; its scales [m, batch, blocks]: one for each row of any view
+    A = A.transpose(0, 1)
+    scale = torch.rand(m, 3, 2, generator=g).cuda().transpose(0, 1)
+    B, sb = ref.random_operand(g, (3, 60, 256), "tiles")
+    out = torch.full((m, 3, 64), 5.0, device="cuda")
+    ctc_amd.scaled_contract(A, scale, B, sb, out=out.transpose(0, 1)[..., :60])
+    check_product(A, scale, B, sb, out.transpose(0, 1)[..., :60], F32)
+    assert bool((out[..., 60:] == 5).all())
+
+
 # ---- groups ----------------------------------------------------------------------------------------------------------
 def offsets_of(counts, first=0):
     return torch.tensor([first] + counts, dtype=torch.int32).cumsum(0).to(torch.int32).cuda()
@@ -333,6 +380,37 @@ def test_groups_of_the_contracted_index(cuda, counts, tail, m, n, dtype):
         want = 0.5 * want - 3.0
         bound = ref.product_bound(want, mag, counts[e] + 1, dtype, 0.5, -1.0, torch.full_like(want, 3.0), dtype is BF16)
         assert bool(((got[e].double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("groups", [64, 65, 200])
+def test_many_groups_of_the_contracted_index(cuda, groups):
+    """Up to 64 groups the longest come first, beyond that in their order; equal lengths and empty groups among them."""
+    g = gen(groups)
+    counts = [128 * int(c) for c in torch.randint(0, 4, (groups,), generator=g)]
+    k = sum(counts)
+    A, sa = ref.random_operand(g, (20, k), "rows")
+    B, sb = ref.random_operand(g, (30, k), "rows")
+    off = offsets_of(counts)
+    got = ctc_amd.scaled_grouped_contract(A, sa, B, sb, off, along="contracted", dtype=F32)
+    at = off.tolist()
+    for e in range(groups):
+        want, mag = ref.product(A, sa, B, sb, at[e], at[e + 1])
+        assert bool(((got[e].double() - want).abs() <= ref.product_bound(want, mag, counts[e] + 1, F32)).all())
+
+
+@pytest.mark.parametrize("bad", [[-300, 128, 256], [256, 128, 512], [0, 1000, 512], [0, 100, 512], [512, 512, 512]])
+def test_contracted_offsets_outside_the_operands_stay_inside(cuda, bad):
+    """Values past the ends count as the ends, falling pairs as empty and others as the block they fall into."""
+    g = gen(22)
+    A, sa = ref.random_operand(g, (40, 512), "rows")
+    B, sb = ref.random_operand(g, (50, 512), "rows")
+    frame = torch.full((4, 40, 50), 5.0, device="cuda")
+    ctc_amd.scaled_grouped_contract(A, sa, B, sb, torch.tensor(bad, dtype=torch.int32, device="cuda"), along="contracted", out=frame[1:3])
+    assert bool((frame[0] == 5).all()) and bool((frame[3] == 5).all())
+    at = [min(max(b, 0), 512) // 128 * 128 for b in bad]
+    for e in range(2):
+        want, mag = ref.product(A, sa, B, sb, at[e], max(at[e], at[e + 1]))
+        assert bool(((frame[1 + e].double() - want).abs() <= ref.product_bound(want, mag, 512, F32)).all())
 
 
 # ---- the experts' layer -------------------------------------------------------------------------------------------------
