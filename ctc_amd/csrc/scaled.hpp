@@ -44,6 +44,7 @@ struct ScaledGemmParams {
     const int32_t *offsets = nullptr;  // grouped: batch + 1 offsets of rows (of contracted elements), on the device
     // schedule
     int nbm = 0, nbn = 0;
+    int cus = 0;  // compute units where the large tile's kernel tells full tiles from light ones, else 0
     int split = 1, steps_per = 0;  // dense: K blocks of a chunk; partial sums of chunk s at ws + s * batch * M * N
     float *ws = nullptr;
 };
@@ -55,7 +56,7 @@ struct ScaledSchedule {
 };
 // cus: compute units of the device; ws_limit: bytes of workspace the caller has
 ScaledSchedule schedule_scaled(const ScaledGemmParams &p, int cus, size_t ws_limit);
-hipError_t launch_scaled_gemm(ScaledGemmParams p, const ScaledSchedule &s, hipStream_t stream);
+hipError_t launch_scaled_gemm(ScaledGemmParams p, const ScaledSchedule &s, int cus, hipStream_t stream);
 hipError_t launch_scaled_skinny(const ScaledGemmParams &p, hipStream_t stream);
 
 // ---- the experts' layer for a few tokens (expert_kernels.hip) ----

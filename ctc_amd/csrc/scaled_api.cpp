@@ -132,9 +132,10 @@ int check_result(const char *what, const void *C, int64_t ldc, int64_t c_batch, 
 int run_product(const char *what, ctc::ScaledGemmParams &p, void *workspace, int64_t workspace_bytes, hipStream_t stream)
 {
     const size_t room = workspace ? (size_t)workspace_bytes : 0;
-    const ctc::ScaledSchedule s = ctc::schedule_scaled(p, compute_units(), room);
+    const int cus = compute_units();
+    const ctc::ScaledSchedule s = ctc::schedule_scaled(p, cus, room);
     p.ws = static_cast<float *>(workspace);
-    hipError_t e = s.kind == 0 ? ctc::launch_scaled_skinny(p, stream) : ctc::launch_scaled_gemm(p, s, stream);
+    hipError_t e = s.kind == 0 ? ctc::launch_scaled_skinny(p, stream) : ctc::launch_scaled_gemm(p, s, cus, stream);
     if (e == hipErrorInvalidValue) return unsupported(what, "too many tiles for one launch");
     if (e != hipSuccess) return set_last_hip_error(e, what);
     (s.kind == 0 ? g_skinny : s.kind == 1 ? g_tile128 : g_tile256).fetch_add(1, std::memory_order_relaxed);

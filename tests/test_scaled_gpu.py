@@ -162,6 +162,30 @@ def test_product_large(cuda, m, n, k, blocks):
     check_product(A, sa, B, sb, got, BF16)
 
 
+# On 256 compute units: full tiles alone, a last round in halves, a light last row, both, several entries, light tiles alone
+@pytest.mark.parametrize("batch, m, n, k", [
+    (1, 2048, 8192, 144), (1, 2304, 8192, 160), (1, 2100, 8192, 400), (1, 2400, 8200, 272), (3, 1500, 4000, 16), (2, 1400, 5000, 656), (1, 100, 60000, 144),
+    (1, 129, 60000, 1296),
+])
+@pytest.mark.parametrize("blocks", [("rows", "tiles"), ("tiles", "rows")])
+@pytest.mark.parametrize("a_dtype", [E4M3, E5M2])
+def test_product_in_full_tiles_halves_and_light_tiles(cuda, batch, m, n, k, blocks, a_dtype):
+    g = gen(m + n + k)
+    A, sa = ref.random_operand(g, (batch, m, k), blocks[0], a_dtype)
+    B, sb = ref.random_operand(g, (batch, n, k), blocks[1])
+    if a_dtype is E5M2:
+        sa = sa * 2.0 ** -7  # e5m2's values reach 2^7 times as far
+    whole = torch.randn(batch, m + 2, n, generator=g).to(BF16).cuda()
+    before = whole.clone()
+    launches = ctc_amd.get_option("launches_scaled_256")
+    # every element once: a second visit would add to it again
+    ctc_amd.scaled_contract(A, sa, B, sb, out=whole[:, 1:-1], alpha=0.5, beta=0.75)
+    assert ctc_amd.get_option("launches_scaled_256") == launches + 1
+    assert torch.equal(whole[:, 0], before[:, 0]) and torch.equal(whole[:, -1], before[:, -1])
+    for b in range(batch):
+        check_product(A[b], sa[b], B[b], sb[b], whole[b, 1:-1], BF16, 0.5, 0.75, before[b, 1:-1])
+
+
 @pytest.mark.parametrize("m", [1, 20, 150, 2500])
 @pytest.mark.parametrize("pitch, shift", [(304, 16), (301, 0), (303, 5), (320, 3), (305, 0)])
 def test_product_alignments(cuda, m, pitch, shift):
@@ -323,6 +347,30 @@ def test_groups_of_rows(cuda, counts, n, k, dtype):
         if counts[e]:
             lo, hi = at[e], at[e + 1]
             check_product(A[lo:hi], sa[lo:hi], B[e], sb[e], out[lo:hi], dtype, fast=rows > 8 * len(counts))
+
+
+@pytest.mark.parametrize("counts", [
+    [2304], [2304, 100], [128, 129, 256, 257, 384, 385, 1, 0, 2000], [100] * 20, [512] * 5 + [0] * 70 + [130], [3, 2800, 5], [1] * 100 + [1500],
+])
+@pytest.mark.parametrize("k", [16, 144, 400, 1040])
+def test_groups_of_rows_in_full_tiles_halves_and_light_tiles(cuda, counts, k):
+    g = gen(sum(counts) + k)
+    rows, n = sum(counts) + 1, 8192
+    A, sa = ref.random_operand(g, (rows, k), "rows")
+    B, sb = ref.random_operand(g, (1, n, k), "tiles")
+    B, sb = B.expand(len(counts), n, k), sb * torch.exp2(torch.arange(len(counts), device="cuda") % 5.0)[:, None, None]
+    out = torch.randn(rows, n, generator=g).to(BF16).cuda()
+    before = out.clone()
+    off = offsets_of(counts)
+    launches = ctc_amd.get_option("launches_scaled_256")
+    ctc_amd.scaled_grouped_contract(A, sa, B, sb, off, out=out, alpha=0.5, beta=0.75)
+    assert ctc_amd.get_option("launches_scaled_256") == launches + 1
+    assert torch.equal(out[-1], before[-1])
+    at = off.tolist()
+    for e in range(len(counts)):
+        lo, hi = at[e], at[e + 1]
+        if hi > lo:
+            check_product(A[lo:hi], sa[lo:hi], B[e], sb[e], out[lo:hi], BF16, 0.5, 0.75, before[lo:hi], fast=True)
 
 
 @pytest.mark.parametrize("blocks", [("rows", "rows"), ("tiles", "tiles")])
