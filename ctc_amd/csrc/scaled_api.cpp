@@ -304,6 +304,8 @@ int ctc_tc_expert_layer(int64_t tokens, int64_t top, int64_t experts, int64_t hi
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 1 || (reinterpret_cast<uintptr_t>(pick) | reinterpret_cast<uintptr_t>(gate)) & 3)
         return set_last_error(CTC_TC_EALIGN, "expert_layer: an argument is not aligned to its elements");
     if (ldx < hidden || ldy < hidden || ld_pick < top || ld_gate < top) return refuse(what, "a leading dimension is below its row length");
+    for (int64_t ld : {ldx, ldy, ld_pick, ld_gate})
+        if (span(1, 0, tokens, ld, hidden) > kMaxSpan) return unsupported(what, "an argument spans too much memory");
     if (!workspace || workspace_bytes < tokens * top * inner * 2) return refuse(what, "the workspace is smaller than expert_workspace_bytes says");
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return set_last_error(CTC_TC_EALIGN, "expert_layer: the workspace is not 16-byte aligned");
     ctc::ExpertParams p;

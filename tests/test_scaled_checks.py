@@ -87,6 +87,7 @@ def test_grouped_product_refuses(kw, code):
     (dict(top=0), EINVAL), (dict(inner=0), EINVAL), (dict(up=matrix()), EUNSUPPORTED), (dict(down=matrix(dtype=_lib.F8E5M2, block=_lib.BLOCK_TILES)), EUNSUPPORTED),
     (dict(x=None), EINVAL), (dict(gate=ADDR + 2), EALIGN), (dict(y=ADDR + 1), EALIGN), (dict(ldx=255), EINVAL), (dict(ld=1), EINVAL),
     (dict(ws=None), EINVAL), (dict(room=2 * 2 * 256 * 2 - 1), EINVAL), (dict(ws=ADDR + 4), EALIGN),
+    (dict(ldx=1 << 60), EUNSUPPORTED), (dict(ldy=1 << 50), EUNSUPPORTED), (dict(ld=1 << 62), EUNSUPPORTED),
 ])
 def test_expert_layer_refuses(kw, code):
     assert experts(**kw) == code
