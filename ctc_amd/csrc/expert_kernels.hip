@@ -73,7 +73,7 @@ __device__ __forceinline__ int place_of(const Picks &k, int e)
 
 // h = gate * silu(G x) * (U x) for 16 of an expert's inner rows and all its tokens.  Workgroup (slice, y): y is a pair
 // (token, place) where there are fewer pairs than experts, and only the first pair of an expert works; else y is the expert.
-// Eight waves share the contracted blocks; their partial sums meet in LDS, in wave order.
+// The waves share the contracted blocks, U in flight each; their partial sums meet in LDS, in wave order.
 template <bool UNI, int NW, int U> __global__ void __launch_bounds__(NW * 64) expert_up_kernel(ExpertParams p, int by_pair)
 {
     __shared__ __attribute__((aligned(16))) float part[NW][2][256];
@@ -295,6 +295,8 @@ hipError_t launch_expert_layer(const ExpertParams &p, hipStream_t stream)
     const int by_pair = pairs < p.experts;
     const dim3 up((unsigned)((p.inner + 15) / 16), (unsigned)(by_pair ? pairs : p.experts));
     const bool uni = p.inner % 16 == 0;
+    // Four waves with two blocks in flight where workgroups abound (32 tokens, 4096 and 1536: 161 us, as with two waves; eight take 172
+    // and more), else eight with one (one token, 2048 and 1024: 11.1 us; four take 11.6, two 12.3)
     if ((int64_t)up.x * up.y >= 2048) {
         if (uni) hipLaunchKernelGGL((expert_up_kernel<true, 4, 2>), up, dim3(4 * 64), 0, stream, p, by_pair);
         else hipLaunchKernelGGL((expert_up_kernel<false, 4, 2>), up, dim3(4 * 64), 0, stream, p, by_pair);

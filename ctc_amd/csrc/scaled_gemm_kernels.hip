@@ -614,14 +614,14 @@ hipError_t launch_scaled_gemm(ScaledGemmParams p, const ScaledSchedule &s, int c
     double count = (double)p.nbm * p.nbn * p.batch * p.split;
     // row tiles of ragged groups: each group adds at most one partly filled tile
     if (p.mode == kScaledRows) count = (double)(p.M / b + (p.batch < p.M ? p.batch : p.M)) * p.nbn;
-    if (count > 0x7fffff) return hipErrorInvalidValue;
+    if (count > 0x7fffff - cus) return hipErrorInvalidValue;  // (512 threads each: a launch holds fewer than 2^32)
     if (s.kind == 2) {
         // Groups always have light tiles (32 groups, 16384 rows, 2048 x 4096: 205 -> 197 us; 64 groups, 4096 rows, 4096 x 2048: 163 -> 140).
         // A dense product may have a light last row or a last round to halve; beyond eight rounds neither pays the full tiles' 1 %.
         const bool light = (p.M - 1) % b < b / 2;
         const int tiles = (int)count, full = light ? tiles / p.nbm * (p.nbm - 1) : tiles, rest = full % cus;
         const bool halves = rest > 0 && 2 * rest + (tiles - full) <= cus;
-        if (p.mode == kScaledRows || ((light || halves) && tiles <= 8 * cus)) {
+        if (p.mode == kScaledRows || (p.mode == kScaledDense && (light || halves) && tiles <= 8 * cus)) {
             p.cus = cus;
             count += cus / 2;  // a tile in halves is one workgroup more
         }

@@ -430,6 +430,25 @@ def test_groups_of_the_contracted_index(cuda, counts, tail, m, n, dtype):
         assert bool(((got[e].double() - want).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("m, n", [(1100, 2048), (2304, 1024), (1536, 2100), (100, 8000)])
+@pytest.mark.parametrize("counts", [[256, 0, 128, 128, 384, 0, 128, 256], [0, 0, 1024, 0, 0, 0, 0, 128]])
+def test_groups_of_the_contracted_index_on_the_large_tile(cuda, m, n, counts):
+    g = gen(m + n + counts[0])
+    k = sum(counts)
+    A, sa = ref.random_operand(g, (m, k), "rows")
+    B, sb = ref.random_operand(g, (n, k), "rows")
+    off = offsets_of(counts)
+    out = torch.randn(len(counts), m, n, generator=g).to(BF16).cuda()
+    before = out.clone()
+    launches = ctc_amd.get_option("launches_scaled_256")
+    ctc_amd.scaled_grouped_contract(A, sa, B, sb, off, along="contracted", out=out, alpha=0.5, beta=0.75)
+    assert ctc_amd.get_option("launches_scaled_256") == launches + 1
+    at = off.tolist()
+    for e in range(len(counts)):
+        lo, hi = at[e], at[e + 1]
+        check_product(A[:, lo:hi], sa[:, lo // 128:hi // 128], B[:, lo:hi], sb[:, lo // 128:hi // 128], out[e], BF16, 0.5, 0.75, before[e], fast=True)
+
+
 @pytest.mark.parametrize("groups", [64, 65, 200])
 def test_many_groups_of_the_contracted_index(cuda, groups):
     """Up to 64 groups the longest come first, beyond that in their order; equal lengths and empty groups among them."""
