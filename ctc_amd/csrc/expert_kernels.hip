@@ -295,18 +295,14 @@ hipError_t launch_expert_layer(const ExpertParams &p, hipStream_t stream)
     const int by_pair = pairs < p.experts;
     const dim3 up((unsigned)((p.inner + 15) / 16), (unsigned)(by_pair ? pairs : p.experts));
     const bool uni = p.inner % 16 == 0;
-    // Four waves with two blocks in flight where workgroups abound (32 tokens, 4096 and 1536: 161 us, as with two waves; eight take 172
-    // and more), else eight with one (one token, 2048 and 1024: 11.1 us; four take 11.6, two 12.3)
-    if ((int64_t)up.x * up.y >= 2048) {
-        if (uni) hipLaunchKernelGGL((expert_up_kernel<true, 4, 2>), up, dim3(4 * 64), 0, stream, p, by_pair);
-        else hipLaunchKernelGGL((expert_up_kernel<false, 4, 2>), up, dim3(4 * 64), 0, stream, p, by_pair);
-    } else {
-        if (uni) hipLaunchKernelGGL((expert_up_kernel<true, 8, 1>), up, dim3(512), 0, stream, p, by_pair);
-        else hipLaunchKernelGGL((expert_up_kernel<false, 8, 1>), up, dim3(512), 0, stream, p, by_pair);
-    }
+    // four waves with two blocks in flight (32 tokens, 4096 and 1536: 161 us, as with two waves; eight take 172 and more.  One token's layer
+    // of 128 experts of 4096 and 1536: 42.6 us; eight waves with one block take 45.9, with two 49.2, sixteen 51.6)
+    if (uni) hipLaunchKernelGGL((expert_up_kernel<true, 4, 2>), up, dim3(4 * 64), 0, stream, p, by_pair);
+    else hipLaunchKernelGGL((expert_up_kernel<false, 4, 2>), up, dim3(4 * 64), 0, stream, p, by_pair);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // at most `pairs` experts: with fewer than the waves, several waves share one expert's contracted blocks
+    // Eight waves with two blocks in flight (sixteen waves, or four blocks: 0 to 1 us more).  At most `pairs` experts: with fewer than the
+    // waves, several waves share one expert's contracted blocks
     int k_parts = 1;
     while (k_parts < 8 && pairs * k_parts < 8) k_parts *= 2;
     hipLaunchKernelGGL((expert_down_kernel<8, 2>), dim3((unsigned)((p.hidden + 15) / 16)), dim3(512), (size_t)8 * p.tokens * 16 * 4, stream, p, k_parts);

@@ -525,24 +525,36 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmP
     multiply_tile<FA, FAST, BUNI, BM, BN, WM, WN, DMA, 2>(p, it, image, scales);
 }
 
-// Sums the chunks' partial results in the order of the chunks (the same on every run) and stores C.
+// Sums the chunks' partial results in the order of the chunks (the same on every run) and stores C.  A split result has fewer
+// tiles than the device compute units, hence indexes of 32 bits.  Four chunks are requested at a time: one by one, each would wait
+// for the one before it.
 __global__ void __launch_bounds__(256) scaled_split_sum_kernel(ScaledGemmParams p)
 {
-    const int64_t per = p.M * p.N, total = per * p.batch;
-    const int64_t quads = (p.N + 3) >> 2, items = quads * p.M * p.batch;
+    const uint32_t rows = (uint32_t)p.M, quads = (uint32_t)((p.N + 3) >> 2), items = quads * rows * (uint32_t)p.batch;
+    const int64_t total = p.M * p.N * p.batch;
     const bool vec = ((p.ldc | p.c_batch) & 3) == 0 && (reinterpret_cast<uintptr_t>(p.C) & (p.c_f32 ? 15 : 7)) == 0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
-        const int64_t n = (i % quads) * 4, rest = i / quads, m = rest % p.M, b = rest / p.M;
-        const float *w = p.ws + b * per + m * p.N + n;
+    const bool whole = (p.N & 3) == 0;
+    for (uint32_t i = blockIdx.x * 256 + threadIdx.x; i < items; i += gridDim.x * 256) {
+        const uint32_t line = i / quads, b = line / rows;
+        const int64_t n = (int64_t)(i - line * quads) * 4, m = line - b * rows;
+        const float *w = p.ws + (int64_t)line * p.N + n;
         v4f v = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < p.split; ++s, w += total) {
-            if ((p.N & 3) == 0) {
-                v += *reinterpret_cast<const v4f *>(w);
-            } else {
+        for (int s0 = 0; s0 < p.split; s0 += 4) {
+            v4f part[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (n + r < p.N) v[r] += w[r];
+            for (int u = 0; u < 4; ++u) {  // beyond the last chunk: that one again, not added
+                const float *from = w + (s0 + u < p.split ? s0 + u : p.split - 1) * total;
+                if (whole) {
+                    part[u] = *reinterpret_cast<const v4f *>(from);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) part[u][r] = from[n + r < p.N ? r : 0];
+                }
             }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = s0 + u < p.split ? v[r] + part[u][r] : v[r];
         }
         store4(p, b * p.c_batch + m * p.ldc + n, n, v, vec);
     }
