@@ -50,7 +50,7 @@ struct ScaledGemmParams {
 };
 
 struct ScaledSchedule {
-    int kind = 0;  // 0 skinny (no LDS staging), 1 the 128 tile, 2 the 256 tile
+    int kind = 0;  // 0 skinny (no LDS staging), 1 the 128 tile, 2 the 256 tile, 3 the 128 tile with three stages
     int split = 1;
     size_t ws_bytes = 0;
 };

@@ -138,7 +138,7 @@ int run_product(const char *what, ctc::ScaledGemmParams &p, void *workspace, int
     hipError_t e = s.kind == 0 ? ctc::launch_scaled_skinny(p, stream) : ctc::launch_scaled_gemm(p, s, cus, stream);
     if (e == hipErrorInvalidValue) return unsupported(what, "too many tiles for one launch");
     if (e != hipSuccess) return set_last_hip_error(e, what);
-    (s.kind == 0 ? g_skinny : s.kind == 1 ? g_tile128 : g_tile256).fetch_add(1, std::memory_order_relaxed);
+    (s.kind == 0 ? g_skinny : s.kind == 2 ? g_tile256 : g_tile128).fetch_add(1, std::memory_order_relaxed);
     if (s.split > 1) g_split.fetch_add(1, std::memory_order_relaxed);
     return CTC_TC_OK;
 }
@@ -210,6 +210,7 @@ int64_t ctc_tc_scaled_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t b
     p.N = n;
     p.K = k;
     p.batch = (int)batch;
+    p.a.ld = 1;  // operands off 16 bytes split the furthest
     return (int64_t)ctc::schedule_scaled(p, compute_units(), (size_t)1 << 62).ws_bytes;
 }
 

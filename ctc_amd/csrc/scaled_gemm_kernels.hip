@@ -236,7 +236,7 @@ __device__ __forceinline__ void store_partial(float *w, int64_t left, v4f v, boo
 // uniform in a wave.  DMA: both operands 16-byte aligned with row pitches that are multiples of 16: their blocks go
 // global -> LDS by DMA; otherwise they pass through registers, requested a block ahead (byte-exact at any alignment).
 //
-// LDS, two stages (light tiles: three) of a block each: rows of 128 bytes, 16-byte chunk c of row r at c ^ (r / 2 & 7).  A fragment is the
+// LDS, two stages (light tiles, and workgroups alone on a CU: three) of a block each: rows of 128 bytes, 16-byte chunk c of row r at c ^ (r / 2 & 7).  A fragment is the
 // chunks g and g + 4 of row l % 16 (g = l / 16), for both operands alike, so that the k order inside the MFMA's block
 // does not matter; with the XOR sixteen lanes that ds_read_b128 serves together fall on sixteen different 16-byte slots.
 //
@@ -503,11 +503,11 @@ __device__ __forceinline__ void multiply_tile(const ScaledGemmParams &p, const I
 // LIGHT: tiles of at most BM / 2 rows run on waves of half the rows; three of their blocks fit in LDS, which is worth another tenth
 // (64 groups, 16384 rows, 2048 x 2048: 165 us without light tiles, 157 with two stages, 150 with three).  A second copy of the kernel,
 // since the other tiles' presence costs the full ones 1 % (4096 x 8192 x 4096).
-template <int FA, bool FAST, bool BUNI, int BM, int BN, int WM, int WN, bool DMA, bool LIGHT>
+template <int FA, bool FAST, bool BUNI, int BM, int BN, int WM, int WN, bool DMA, bool LIGHT, int STAGES>
 __global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmParams p)
 {
-    __shared__ __attribute__((aligned(16))) uint8_t image[LIGHT ? 3 * (BM / 2 + BN) * 128 : 2 * (BM + BN) * 128];
-    __shared__ __attribute__((aligned(16))) float scales[LIGHT ? 3 * (BM / 2 + BN) + 128 : 2 * (BM + BN)];
+    __shared__ __attribute__((aligned(16))) uint8_t image[LIGHT ? 3 * (BM / 2 + BN) * 128 : STAGES * (BM + BN) * 128];
+    __shared__ __attribute__((aligned(16))) float scales[LIGHT ? 3 * (BM / 2 + BN) + 128 : STAGES * (BM + BN)];
     Item it;
     if (!find_item<BM, BN, LIGHT>(p, it)) return;
     it.m0 = uniform(it.m0);
@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmP
             return;
         }
     }
-    multiply_tile<FA, FAST, BUNI, BM, BN, WM, WN, DMA, 2>(p, it, image, scales);
+    multiply_tile<FA, FAST, BUNI, BM, BN, WM, WN, DMA, STAGES>(p, it, image, scales);
 }
 
 // Sums the chunks' partial results in the order of the chunks (the same on every run) and stores C.  A split result has fewer
@@ -565,16 +565,18 @@ template <int FA, bool FAST, bool BUNI> hipError_t launch_tiles(const ScaledGemm
     if constexpr (FAST) {  // (two fragments of bf16 do not fit the registers beside 128 accumulators)
         if (kind == 2) {
             if (p.cus > 0)
-                hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 256, 256, 2, 4, true, true>), dim3(grid), dim3(512), 0, stream, p);
+                hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 256, 256, 2, 4, true, true, 2>), dim3(grid), dim3(512), 0, stream, p);
             else
-                hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 256, 256, 2, 4, true, false>), dim3(grid), dim3(512), 0, stream, p);
+                hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 256, 256, 2, 4, true, false, 2>), dim3(grid), dim3(512), 0, stream, p);
             return hipGetLastError();
         }
     }
-    if (dma)
-        hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 128, 128, 2, 2, true, false>), dim3(grid), dim3(256), 0, stream, p);
+    if (dma && kind == 3)
+        hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 128, 128, 2, 2, true, false, 3>), dim3(grid), dim3(256), 0, stream, p);
+    else if (dma)
+        hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 128, 128, 2, 2, true, false, 2>), dim3(grid), dim3(256), 0, stream, p);
     else
-        hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 128, 128, 2, 2, false, false>), dim3(grid), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((scaled_gemm_kernel<FA, FAST, BUNI, 128, 128, 2, 2, false, false, 2>), dim3(grid), dim3(256), 0, stream, p);
     return hipGetLastError();
 }
 
@@ -601,7 +603,10 @@ ScaledSchedule schedule_scaled(const ScaledGemmParams &p, int cus, size_t ws_lim
         const int64_t steps = (p.K + kScaleBlock - 1) / kScaleBlock;
         // chunks of eight blocks or more, 64 at most: a second launch has to pay (150 x 260 x 16384: 20 us in chunks of four, 16 of
         // eight, 18 of sixteen, 84 whole; 128 x 128 x 131072: 80 in 256 chunks, 47 in 128, 35 in 64, 614 whole)
-        int64_t split = (int64_t)(2 * cus / tiles(128));
+        // With DMA one workgroup a compute unit and three stages: longer chunks, fewer partial sums (512 x 4096 x 4096: 26.1 -> 23.3 us;
+        // 128 x 8192 x 8192: 31.0 -> 26.3; 48 x 4096 x 4096: 13.2 -> 12.8); without, two workgroups.
+        const bool dma = dma_ready(p.a, p.K) && dma_ready(p.b, p.K);
+        int64_t split = (int64_t)((dma ? 1 : 2) * cus / tiles(128));
         if (split > steps / 8) split = steps / 8;
         if (split > 64) split = 64;
         const size_t one = (size_t)p.M * p.N * p.batch * 4;
@@ -611,6 +616,7 @@ ScaledSchedule schedule_scaled(const ScaledGemmParams &p, int cus, size_t ws_lim
             s.split = (int)((steps + per - 1) / per);
             s.ws_bytes = s.split > 1 ? (size_t)s.split * one : 0;
         }
+        if (dma && tiles(128) * s.split <= cus) s.kind = 3;
     }
     return s;
 }

@@ -137,7 +137,7 @@ def test_kernels_that_set_m0_from_assembly_have_no_other_m0_user(tmp_path):
                 assert not re.match(r"s_mov_b32 m0", before), (name, before, last, inst)
                 assert "m0" not in inst or re.match(r"s_mov_b32 m0, s\d+$", inst), (name, inst)
             before, last = last, inst
-    assert len(kernels) == 16, kernels  # two types of A, two of scales: two forms of the large tile, two sums on the small one
+    assert len(kernels) == 24, kernels  # two types of A, two of scales: two forms of the large tile, two sums and two depths on the small one
 
 
 def test_nothing_to_do_succeeds_without_a_device():
