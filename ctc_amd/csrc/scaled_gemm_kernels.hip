@@ -504,7 +504,7 @@ __device__ __forceinline__ void multiply_tile(const ScaledGemmParams &p, const I
 // (64 groups, 16384 rows, 2048 x 2048: 165 us without light tiles, 157 with two stages, 150 with three).  A second copy of the kernel,
 // since the other tiles' presence costs the full ones 1 % (4096 x 8192 x 4096).
 template <int FA, bool FAST, bool BUNI, int BM, int BN, int WM, int WN, bool DMA, bool LIGHT, int STAGES>
-__global__ void __launch_bounds__(WM *WN * 64, 2) scaled_gemm_kernel(ScaledGemmParams p)
+__global__ void __launch_bounds__(WM *WN * 64, STAGES > 2 ? 1 : 2) scaled_gemm_kernel(ScaledGemmParams p)
 {
     __shared__ __attribute__((aligned(16))) uint8_t image[LIGHT ? 3 * (BM / 2 + BN) * 128 : STAGES * (BM + BN) * 128];
     __shared__ __attribute__((aligned(16))) float scales[LIGHT ? 3 * (BM / 2 + BN) + 128 : STAGES * (BM + BN)];
