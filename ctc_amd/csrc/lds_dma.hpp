@@ -43,7 +43,7 @@ __device__ __forceinline__ void dma16_split(const void *uniform_base, unsigned l
 }
 
 // The same with the wait state that the instruction set asks for between a write of M0 and a transfer that reads it (no
-// measurable cost: 4096 x 8192 x 4096 of the block-scaled products takes 136 us either way).
+// measurable cost: a transfer's wave waits for its turn in any case).
 __device__ __forceinline__ void dma16_spaced(const void *uniform_base, unsigned lane_offset, unsigned lds_wave_base)
 {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
