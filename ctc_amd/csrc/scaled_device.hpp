@@ -64,6 +64,19 @@ template <int FA, bool FAST, int NT> __device__ __forceinline__ void block_sums(
     }
 }
 
+// The product of a block's two scales as f * 2^e, f of 1 to 4 in magnitude: as one f32 number it can be subnormal or infinite
+// (scales of 2^-109 and 2^-30, of 2^64 and 2^100) where the block's term is neither.  Zeros, infinities and NaNs stay in f.
+struct ScalePair {
+    float f;
+    int e;
+};
+__device__ __forceinline__ ScalePair scale_pair(float sa, float sb)
+{
+    return {4.f * (__builtin_amdgcn_frexp_mantf(sa) * __builtin_amdgcn_frexp_mantf(sb)), __builtin_amdgcn_frexp_expf(sa) + __builtin_amdgcn_frexp_expf(sb) - 2};
+}
+// acc + d * f * 2^e.  A power of two scales d without rounding, so these are the bits of fma(d, sa * sb, acc) wherever sa * sb is a normal number.
+__device__ __forceinline__ float add_scaled(float d, ScalePair s, float acc) { return __builtin_fmaf(__builtin_ldexpf(d, s.e), s.f, acc); }
+
 __device__ __forceinline__ v4i load16(const uint8_t *q)  // any alignment
 {
     v4i v;

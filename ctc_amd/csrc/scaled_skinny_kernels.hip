@@ -57,6 +57,7 @@ template <int FA, bool BUNI, int MT, int NW, int U> __global__ void __launch_bou
         v4f acc[MT];
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        bool odd = false;  // a product of scales is no normal number
         // `mine` chooses and does not branch: loads would sink into the branches, one wait each
         auto multiply = [&](const Codes &cb, const Codes(&ca)[MT], const float(&sb)[S], const float(&sa)[MT], bool mine) {
             BlockOperand<0, false> ob[1];
@@ -67,8 +68,14 @@ template <int FA, bool BUNI, int MT, int NW, int U> __global__ void __launch_bou
                 oa.set(ca[i].lo, ca[i].hi);
                 v4f d[1];
                 block_sums<FA, false, 1>(ob, oa, d);
+                float f[S];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[i][r] = mine ? __builtin_fmaf(d[0][r], sa[i] * sb[BUNI ? 0 : r], acc[i][r]) : acc[i][r];
+                for (int r = 0; r < S; ++r) {
+                    f[r] = sa[i] * sb[r];
+                    odd |= !__builtin_isnormal(f[r]);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][r] = mine ? __builtin_fmaf(d[0][r], f[BUNI ? 0 : r], acc[i][r]) : acc[i][r];
             }
         };
         for (int s0 = wave; s0 < whole; s0 += NW * U) {
@@ -93,18 +100,37 @@ template <int FA, bool BUNI, int MT, int NW, int U> __global__ void __launch_bou
                 multiply(tb, ta, sb[u], sa[u], s0 + u * NW < whole);
             }
         }
-        if (p.K % kScaleBlock != 0 && wave == whole % NW) {  // the block that K ends in
-            const int64_t k = (int64_t)whole * kScaleBlock;
-            Codes cb = load_last_codes(B + min64(n0 + fr, p.N - 1) * p.b.ld + fg * 16, k, p.K - fg * 16, p.K >= 16), ca[MT];
-            float sb[S], sa[MT];
+        // The block that K ends in; and where a product of scales was no normal number all of the wave's blocks once more: with the scales'
+        // exponents apart from their product
+        const bool again = __ballot(odd) != 0;
+        if (__builtin_expect(again, 0)) {
 #pragma unroll
-            for (int r = 0; r < S; ++r) sb[r] = sb_ptr[r][whole * p.b.s_blk];
+            for (int i = 0; i < MT; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        const int blocks = (int)((p.K + kScaleBlock - 1) / kScaleBlock);
+#pragma unroll 1
+        for (int s = again ? wave : wave == whole % NW ? whole : blocks; s < blocks; s += NW) {
+            int l = lane;
+            asm volatile("" : "+v"(l));  // addresses made here: held in front of the loop they cost the one above its registers
+            const int row = l & 15, col = (l >> 4) * 16;
+            const int64_t k = (int64_t)s * kScaleBlock, k_end = p.K - col;
+            BlockOperand<0, false> ob[1];
+            const Codes cb = load_last_codes(B + min64(n0 + row, p.N - 1) * p.b.ld + col, k, k_end, p.K >= 16);
+            ob[0].set(cb.lo, cb.hi);
+            float sb[S];
+#pragma unroll
+            for (int r = 0; r < S; ++r) sb[r] = sb_ptr[r][s * p.b.s_blk];
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                ca[i] = load_last_codes(A + min64(m0 + i * 16 + fr, m_end - 1) * p.a.ld + fg * 16, k, p.K - fg * 16, p.K >= 16);
-                sa[i] = sa_ptr[i][whole * p.a.s_blk];
+                const Codes ca = load_last_codes(A + min64(m0 + i * 16 + row, m_end - 1) * p.a.ld + col, k, k_end, p.K >= 16);
+                const float sa = sa_ptr[i][s * p.a.s_blk];
+                BlockOperand<FA, false> oa;
+                oa.set(ca.lo, ca.hi);
+                v4f d[1];
+                block_sums<FA, false, 1>(ob, oa, d);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][r] = add_scaled(d[0][r], scale_pair(sa, sb[BUNI ? 0 : r]), acc[i][r]);
             }
-            multiply(cb, ca, sb, sa, true);
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) *reinterpret_cast<v4f *>(&part[wave][(i * 16 + fr) * 16 + fg * 4]) = acc[i];
