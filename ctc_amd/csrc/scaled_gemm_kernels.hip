@@ -285,11 +285,13 @@ __device__ __forceinline__ void multiply_tile(const ScaledGemmParams &p, const I
 #pragma unroll
             for (int i = 0; i < NB; ++i) lds_dma::dma16_spaced(B + s * kScaleBlock, b_off[i], base + BM * 128 + i * (T * 16));
         } else {
+            int row = srow;
+            asm volatile("" : "+v"(row));  // each row's address anew: eight of them held through the loop spill
             const int64_t k = s * kScaleBlock + schunk * 16;
 #pragma unroll
-            for (int i = 0; i < NA; ++i) held[i] = load16(A + (int64_t)min(srow + i * (T / 8), a_last) * p.a.ld + k);
+            for (int i = 0; i < NA; ++i) held[i] = load16(A + (int64_t)min(row + i * (T / 8), a_last) * p.a.ld + k);
 #pragma unroll
-            for (int i = 0; i < NB; ++i) held[NA + i] = load16(B + (int64_t)min(srow + i * (T / 8), b_last) * p.b.ld + k);
+            for (int i = 0; i < NB; ++i) held[NA + i] = load16(B + (int64_t)min(row + i * (T / 8), b_last) * p.b.ld + k);
         }
     };
     // without DMA: the block that stage() requested, into LDS
