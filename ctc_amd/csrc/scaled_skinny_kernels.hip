@@ -150,12 +150,19 @@ template <int FA, bool BUNI, int MT, int NW, int U> __global__ void __launch_bou
 // Waves of a workgroup: two where there are workgroups enough and K is short (a wave then has eight blocks or more of its
 // own, and less of its life goes into starting and into the sum over the waves: 64 groups, 96 rows, 2048 x 2048 weights
 // 45 -> 32 us, 4096 x 1024 ones 80 -> 32), eight where there are few workgroups or K is long (1 x 4096 x 8192: 12 us against 17).
-template <int FA, bool BUNI> void launch_b(const ScaledGemmParams &p, unsigned grid, hipStream_t stream)
+struct SkinnyForm {
+    bool two_waves, two_row_tiles;
+};
+SkinnyForm choose_form(const ScaledGemmParams &p)
 {
     const int64_t rows = p.mode == kScaledRows ? (p.M + p.batch - 1) / p.batch : p.M;
-    const int64_t blocks = p.K / kScaleBlock;
-    const bool two = (grid >= 1024 && blocks <= 32) || (grid >= 512 && blocks <= 16);
-    if (rows > 16) {
+    const int64_t grid = (p.N + 15) / 16 * p.batch, blocks = p.K / kScaleBlock;
+    return {(grid >= 1024 && blocks <= 32) || (grid >= 512 && blocks <= 16), rows > 16};
+}
+template <int FA, bool BUNI> void launch_b(const ScaledGemmParams &p, SkinnyForm form, unsigned grid, hipStream_t stream)
+{
+    const bool two = form.two_waves;
+    if (form.two_row_tiles) {
         if (two) hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, 2, 2, 2>), dim3(grid), dim3(128), 0, stream, p);
         else hipLaunchKernelGGL((scaled_skinny_kernel<FA, BUNI, 2, 8, 2>), dim3(grid), dim3(512), 0, stream, p);
     } else {
@@ -164,23 +171,55 @@ template <int FA, bool BUNI> void launch_b(const ScaledGemmParams &p, unsigned g
     }
 }
 
-}  // namespace
-
-hipError_t launch_scaled_skinny(const ScaledGemmParams &pp, hipStream_t stream)
+// one launch
+hipError_t launch_part(ScaledGemmParams p, SkinnyForm form, hipStream_t stream)
 {
-    ScaledGemmParams p = pp;
     p.nbn = (int)((p.N + 15) / 16);
-    const int64_t grid = (int64_t)p.nbn * p.batch;
-    if (grid > 0x3fffff) return hipErrorInvalidValue;
+    const unsigned grid = (unsigned)p.nbn * (unsigned)p.batch;
     const bool uni = p.b.shift == 7;
     if (p.a.e5m2) {
-        if (uni) launch_b<1, true>(p, (unsigned)grid, stream);
-        else launch_b<1, false>(p, (unsigned)grid, stream);
+        if (uni) launch_b<1, true>(p, form, grid, stream);
+        else launch_b<1, false>(p, form, grid, stream);
     } else {
-        if (uni) launch_b<0, true>(p, (unsigned)grid, stream);
-        else launch_b<0, false>(p, (unsigned)grid, stream);
+        if (uni) launch_b<0, true>(p, form, grid, stream);
+        else launch_b<0, false>(p, form, grid, stream);
     }
     return hipGetLastError();
+}
+
+}  // namespace
+
+// A launch holds fewer than 2^32 threads, of which a workgroup has up to 512: entries beyond 2^22 workgroups, and columns beyond as many,
+// take launches of their own, all of one form.
+hipError_t launch_scaled_skinny(const ScaledGemmParams &p, hipStream_t stream)
+{
+    constexpr int64_t kMostGroups = 0x3fffff, kMostColumns = kMostGroups * 16 / kScaleBlock * kScaleBlock;  // whole tiles of B's scales
+    const SkinnyForm form = choose_form(p);
+    const int64_t size = p.c_f32 ? 4 : 2;
+    for (int64_t n0 = 0; n0 < p.N; n0 += kMostColumns) {
+        ScaledGemmParams columns = p;
+        columns.N = p.N - n0 < kMostColumns ? p.N - n0 : kMostColumns;
+        columns.b.q += n0 * p.b.ld;
+        columns.b.scale += (n0 >> p.b.shift) * p.b.s_row;
+        columns.C = static_cast<char *>(p.C) + n0 * size;
+        const int64_t entries = kMostGroups / ((columns.N + 15) / 16);
+        for (int64_t e = 0; e < p.batch; e += entries) {
+            ScaledGemmParams part = columns;
+            part.batch = (int)(p.batch - e < entries ? p.batch - e : entries);
+            part.b.q += e * p.b.batch;
+            part.b.scale += e * p.b.s_batch;
+            if (p.mode == kScaledRows) {
+                part.offsets += e;
+            } else {
+                part.a.q += e * p.a.batch;
+                part.a.scale += e * p.a.s_batch;
+                part.C = static_cast<char *>(columns.C) + e * p.c_batch * size;
+            }
+            const hipError_t err = launch_part(part, form, stream);
+            if (err != hipSuccess) return err;
+        }
+    }
+    return hipSuccess;
 }
 
 }  // namespace ctc
