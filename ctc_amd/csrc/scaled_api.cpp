@@ -203,7 +203,10 @@ int ctc_tc_block_quantize(const void *x, int64_t rows, int64_t cols, int64_t ldx
 
 int64_t ctc_tc_scaled_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t batch)
 {
-    if (m < 0 || n < 0 || k < 0 || batch < 0 || m > kMaxDim || n > kMaxDim || k > kMaxDim || batch > 65535) return CTC_TC_EINVAL;
+    CTC_ABI_TRY
+    const char *what = "scaled_workspace_bytes";
+    if (m < 0 || n < 0 || k < 0 || batch < 0) return refuse(what, "negative size");
+    if (m > kMaxDim || n > kMaxDim || k > kMaxDim || batch > 65535) return unsupported(what, "an extent is too large");
     if (m == 0 || n == 0 || batch == 0) return 0;
     ctc::ScaledGemmParams p;
     p.M = m;
@@ -212,6 +215,7 @@ int64_t ctc_tc_scaled_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t b
     p.batch = (int)batch;
     p.a.ld = 1;  // operands off 16 bytes split the furthest
     return (int64_t)ctc::schedule_scaled(p, compute_units(), (size_t)1 << 62).ws_bytes;
+    CTC_ABI_CATCH
 }
 
 int ctc_tc_scaled_contract(int64_t m, int64_t n, int64_t k, int64_t batch, const ctc_tc_scaled_matrix *a, const ctc_tc_scaled_matrix *b,
@@ -283,8 +287,14 @@ int ctc_tc_scaled_grouped_contract(int along, int64_t groups, const int32_t *off
 
 int64_t ctc_tc_expert_workspace_bytes(int64_t tokens, int64_t top, int64_t inner)
 {
-    if (tokens < 0 || top < 0 || inner < 0 || tokens > ctc::kExpertMaxTokens || top > ctc::kExpertMaxTop || inner > kMaxDim) return CTC_TC_EINVAL;
+    CTC_ABI_TRY
+    const char *what = "expert_workspace_bytes";
+    if (tokens < 0 || top < 0 || inner < 0) return refuse(what, "negative size");
+    if (tokens > ctc::kExpertMaxTokens) return refuse(what, "at most 64 tokens");
+    if (top > ctc::kExpertMaxTop) return refuse(what, "at most 16 experts a token");
+    if (inner > kMaxDim) return refuse(what, "an extent is too large");
     return tokens * top * inner * 2;
+    CTC_ABI_CATCH
 }
 
 int ctc_tc_expert_layer(int64_t tokens, int64_t top, int64_t experts, int64_t hidden, int64_t inner, const void *x, int64_t ldx,

@@ -224,8 +224,8 @@ def scaled_contract(A, scale_a, B, scale_b, out=None, dtype=None, alpha=1.0, bet
 
     def call(raw):
         c, code, ldc, stride = _result(st, out, lead + (m, n), dtype or st.bf16, device)
-        # (32: products of so few rows never split)
-        room = check(st.lib.ctc_tc_scaled_workspace_bytes(m, n, k, batch)) if m > 32 else 0
+        # (32: products of so few rows never split; a negative answer: the operator refuses the sizes too, with its own words)
+        room = max(st.lib.ctc_tc_scaled_workspace_bytes(m, n, k, batch), 0) if m > 32 else 0
         ws = st.empty(room, dtype=st.torch.uint8, device=device) if room else None
         check(st.lib.ctc_tc_scaled_contract(m, n, k, batch, _byref(a), _byref(b), float(alpha), float(beta), c.data_ptr(), ldc, stride, code,
                                             ws.data_ptr() if room else None, room, raw))
@@ -302,10 +302,10 @@ def expert_layer(x, up, scale_up, down, scale_down, pick, gate, out=None, stream
 
     def call(raw):
         y, _, ldy, _ = _result(st, out, shape, st.bf16, device)
-        room = check(st.lib.ctc_tc_expert_workspace_bytes(tokens, top, inner))
-        ws = st.empty(max(room, 1), dtype=st.torch.uint8, device=device)
+        room = max(st.lib.ctc_tc_expert_workspace_bytes(tokens, top, inner), 1)  # (negative: as in scaled_contract)
+        ws = st.empty(room, dtype=st.torch.uint8, device=device)
         check(st.lib.ctc_tc_expert_layer(tokens, top, experts, hidden, inner, x.data_ptr(), ldx, _byref(u), _byref(d), pick.data_ptr(), ld_pick,
-                                         gate.data_ptr(), ld_gate, y.data_ptr(), ldy, ws.data_ptr(), max(room, 1), raw))
+                                         gate.data_ptr(), ld_gate, y.data_ptr(), ldy, ws.data_ptr(), room, raw))
         return y
 
     return _run(st, device, stream, call)
