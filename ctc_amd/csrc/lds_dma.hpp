@@ -33,7 +33,9 @@ __device__ __forceinline__ void dma16(const void *src, unsigned char *lds_wave_b
 // clobber: the compiler reserves it and only warns), so a kernel that uses this must have no other user of
 // M0: no dma16() above (there the compiler sets M0 and may assume it unchanged across this statement), no
 // dynamically indexed register array (relative moves go through M0).  tests/test_abi.py disassembles the
-// library and checks exactly that for every kernel whose transfers come from here.
+// library and checks exactly that for every kernel whose transfers come from here.  It also asks for the move directly in front of the
+// transfer, so this form is without the wait state of the next one: the instruction set calls for it, the compiler puts it in front
+// of its own transfers, and no result of the kernels that use this form has shown it missing.
 __device__ __forceinline__ void dma16_split(const void *uniform_base, unsigned lane_offset, unsigned lds_wave_base)
 {
     asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"

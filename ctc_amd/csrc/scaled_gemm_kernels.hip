@@ -121,7 +121,7 @@ __device__ __forceinline__ int longest_first(const int32_t *offsets, int groups,
 
 // The order of the large tile's kernel where it tells full tiles from light ones (at most BM / 2 rows, two thirds of a full one's
 // time): the full ones, then, if the last round of full tiles would keep less than half of the compute units busy, its tiles in halves
-// (4096 x 5120 x 4096, 320 tiles: 125 -> 104 us), then the light ones (4200 x 4096 x 4096: 123 -> 101).
+// (4096 x 5120 x 4096, 320 tiles: 125 -> 106 us), then the light ones (4200 x 4096 x 4096: 123 -> 103).
 struct Place {
     uint32_t id;
     int kind;  // -1 nothing, 0 full, 1 upper half, 2 lower half, 3 light

@@ -110,7 +110,8 @@ template <typename R> __device__ __forceinline__ uint32_t max16(uint32_t m)
 }
 
 // One scale per row and 128 columns, no transpose: sixteen lanes own a group and load it whole (16 or 32 bytes a lane),
-// so the maximum is four exchanges inside sixteen lanes and nothing passes through LDS.
+// so the maximum is four exchanges inside sixteen lanes and nothing passes through LDS.  bf16: 8192 x 4096 28.6 us, 3.5 TB/s,
+// 4096 x 8192 25.7 us; 512 x 4096 and below the call's 8 to 9 us.
 template <int SRC, int FMT> __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantizeParams p, int64_t nblk, int64_t total)
 {
     typedef Row8<SRC> R;

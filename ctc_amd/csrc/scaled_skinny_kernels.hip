@@ -3,7 +3,8 @@
 //
 // A workgroup owns 16 columns of C (rows of B); its waves take the blocks of 128 contracted elements in turn, two or four
 // in flight each, hold the operands in registers (turned through LDS of the wave's own: see Codes) and meet once, in the
-// sum of their partial results, in wave order: the same bits on every run.  1 x 131072 x 8192: 163 us, 6.6 TB/s; 16 rows x 131072 x
+// sum of their partial results, in wave order: the same bits on every run.  A wave that met a product of scales outside the normal
+// numbers takes its blocks once more (see ScalePair); looking costs nothing up to 16 rows and 4 % at 32 x 8192 x 8192 (16.6 -> 17.5 us).  1 x 131072 x 8192: 163 us, 6.6 TB/s; 16 rows x 131072 x
 // 4096: 114 us, 4.7 TB/s (A is as many bytes as B for every workgroup then, out of the L2).
 #include "scaled_device.hpp"
 
@@ -148,8 +149,9 @@ template <int FA, bool BUNI, int MT, int NW, int U> __global__ void __launch_bou
 }
 
 // Waves of a workgroup: two where there are workgroups enough and K is short (a wave then has eight blocks or more of its
-// own, and less of its life goes into starting and into the sum over the waves: 64 groups, 96 rows, 2048 x 2048 weights
-// 45 -> 32 us, 4096 x 1024 ones 80 -> 32), eight where there are few workgroups or K is long (1 x 4096 x 8192: 12 us against 17).
+// own, and less of its life goes into starting and into the sum over the waves: 64 groups, 96 rows spread over them, 2048 x 2048 weights
+// 66 -> 38 us, 4096 x 1024 ones 112 -> 36), eight where there are few workgroups or K is long (1 x 4096 x 8192: 10.5 us against 14.0,
+// 1 x 131072 x 8192: 163 against 184).
 struct SkinnyForm {
     bool two_waves, two_row_tiles;
 };
