@@ -383,6 +383,8 @@ int ctc_tc_grouped_contract(const ctc_tc_small_gemm *problems, int count, int dt
  * The scales' strides are free; the quantiser's callers usually keep the row index fastest (scale_row = 1), which is
  * how the products read them.  No entry point below allocates or synchronises: all may be captured in a HIP graph, and
  * calls on different streams may overlap unless they share a result or a workspace.  Results must not overlap operands.
+ * Limits (CTC_TC_EUNSUPPORTED beyond): extents of 2^31 - 4097, batches and groups of 65535, operands that span 2^46
+ * elements, a quantised matrix of 2^23 blocks of 128 x 128.
  */
 enum ctc_tc_block { CTC_TC_BLOCK_ROWS = 0, CTC_TC_BLOCK_TILES = 1 };
 
